@@ -3,7 +3,8 @@
  *
  * Every entry point takes plain device pointers, element strides and sizes, enqueues its
  * work on the given CUDA stream (passed as void*, a cudaStream_t; NULL = legacy default
- * stream) and returns an rkv_status.  Nothing here allocates, frees or synchronises: the
+ * stream) and returns an rkv_status.  Nothing here allocates, frees or synchronises
+ * (rkv_ragged_error, which reads an error word back, waits for the device): the
  * caller owns every buffer, including the workspaces whose sizes the *_workspace_size
  * queries report, and all sizes needed for a launch are host-known.  Calls are
  * stream-ordered; the library keeps no per-call state, so calls from several host threads
@@ -435,6 +436,68 @@ int rkv_reindex_batch(const rkv_kv_layout* src, const rkv_salience* src_sal,
                       const rkv_kv_layout* dst, const rkv_salience* dst_sal,
                       const int64_t* index, const int64_t* slots, int64_t num_listed,
                       int64_t num_moved, int* err, void* stream);
+
+/* ---- requests of different lengths over one page pool ---------------------------------------
+ * No counterpart in the reference, whose cache holds one length for the whole batch.  The pool
+ * is [num_slots, Hkv, P, D] for each of K and V of a layer (rkv_kv_layout with stride_p,
+ * stride_h, stride_t and num_slots; stride_b and row_map are not used), and every request has
+ * a row of a page table [requests, pt_width] int64 (page_table, pt_stride_b) and its own
+ * length in device memory.  One table serves every layer.  A slot-map entry is
+ * page * P + row in page.
+ *
+ * What a launch finds wrong on the device (a page id outside the pool, a length outside the
+ * table, a step that cannot be granted) is kept in an error word of the library on that
+ * device, not in a workspace: rkv_ragged_error reads it.  These calls need no zeroed memory,
+ * and calls whose buffers are their own may run at the same time. */
+
+/* Page tables and slot map of a step.  Request r holds lengths[r] tokens and is to hold
+ * new_lengths[r].  A request that grows takes pages for the tokens its pages do not hold yet
+ * from the ring of free pages (in request order, from its head) and enters them in its row;
+ * one that shrinks (0: it leaves) gives back the pages behind its new end, in request order,
+ * behind the ring's tail: they can be taken from the next call on, and their table entries
+ * stay as they are.  ring holds ring_size = num_slots page ids; state is int64[3] {head,
+ * count, 0}: ring[(head + i) % ring_size], i < count, are free.
+ *   out_lengths[r]   new_lengths[r]
+ *   out_state        the ring's state after the call
+ *   token_starts     [requests + 1] exclusive sum of the requests' new tokens
+ *   slot_map[i]      slot of the i-th new token (request by request), -1 past the last one
+ *   positions[i]     its position in its request, 0 past the last one
+ * The call is granted as a whole or refused as a whole, with error 4 in the error word:
+ * pages missing, more than max_new_tokens new tokens, a length outside [0, pt_width * P], more
+ * pages given back than the ring holds, or a state that is none.  Refused, out_lengths are
+ * lengths, out_state is state, and every slot is -1.  out_lengths may be lengths or
+ * new_lengths, and out_state may be state; page_table and ring are updated in place, in
+ * entries that lengths and state do not cover, so a repeated call gives the same results. */
+int rkv_ragged_page_tables(const int64_t* lengths, const int64_t* new_lengths, int64_t requests,
+                           int64_t page_size, int64_t* page_table, int64_t pt_stride,
+                           int64_t pt_width, int64_t* ring, int64_t ring_size, int64_t* state,
+                           int64_t* out_lengths, int64_t* out_state, int64_t* slot_map,
+                           int64_t* positions, int64_t max_new_tokens, int64_t* token_starts,
+                           void* stream);
+
+/* Writes row t of k_new / v_new [n_new, Hkv, D] (element strides new_stride_t and
+ * new_stride_h) to the pool's slot slot_map[t].  Negative slots are skipped; one past the pool
+ * is skipped with error 2.  Two rows of one slot: either may be the one that stays. */
+int rkv_ragged_append(const rkv_kv_layout* pool, const void* k_new, const void* v_new,
+                      int64_t new_stride_t, int64_t new_stride_h, int64_t n_new,
+                      const int64_t* slot_map, void* stream);
+
+/* out[b, h] = softmax(q . k * scale) . v over the tokens starts[b] <= t < lengths[b] of request b
+ * (starts == NULL: from the first), and lse[b * Hq + h] = log sum exp(q . k * scale) (natural,
+ * fp32; may be NULL).  A request without such a token gives zeros and -inf, and what the pool
+ * holds outside the tokens (NaN included) has no effect.  pool->batch is the number of
+ * requests and pool->num_tokens the table's capacity, pt_width * P.  scale == 0 selects
+ * 1/sqrt(D).  q, pool and out share a dtype; q_len is 1.  A length outside [0, capacity] is
+ * read as the nearer bound with error 3, a page id outside the pool as page 0 with error 2. */
+size_t rkv_ragged_decode_attention_workspace_size(const rkv_query* q, const rkv_kv_layout* pool);
+int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
+                                const int64_t* lengths, const int64_t* starts, float scale,
+                                const rkv_output* out, float* lse, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* Waits for the current device, reads the ragged calls' error word there (0: none; the largest
+ * code otherwise) and, with clear != 0, resets it. */
+int rkv_ragged_error(int clear, int* code);
 
 #ifdef __cplusplus
 }

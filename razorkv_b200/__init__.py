@@ -7,6 +7,8 @@ Public surface (names as in the reference package ``razorkv``):
 * ``RazorEngine`` (HF model patcher; paged attention interface) razorkv/engine.py
 * ``kernels``: ``triton_paged_sparse_attention``, ``compacted_paged_sdpa``,
   ``compute_page_salience_pool``, ``is_triton_available``   razorkv/kernels/
+* ``ragged_page_tables``, ``ragged_append``, ``ragged_decode_attention``: requests of different
+  lengths that share one page pool (no counterpart in the reference)
 
 The CUDA library (librazorkv_b200.so, C ABI in include/razorkv_b200.h) is loaded on first
 use; build it with ``python -m razorkv_b200.build``.
@@ -22,6 +24,13 @@ from .kernels import (
     is_triton_available,
     paged_sparse_attention,
     triton_paged_sparse_attention,
+)
+from .ragged import (
+    RaggedTables,
+    ragged_append,
+    ragged_decode_attention,
+    ragged_free_ring,
+    ragged_page_tables,
 )
 
 __version__ = "0.1.0"
@@ -39,5 +48,10 @@ __all__ = [
     "is_triton_available",
     "paged_sparse_attention",
     "triton_paged_sparse_attention",
+    "RaggedTables",
+    "ragged_append",
+    "ragged_decode_attention",
+    "ragged_free_ring",
+    "ragged_page_tables",
     "__version__",
 ]

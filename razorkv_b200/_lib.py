@@ -131,6 +131,15 @@ _SIGNATURES = {
     "rkv_select_compact_pages": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64,
                                                 c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_sz,
                                                 c_vp]),
+    "rkv_ragged_page_tables": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp,
+                                              c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp,
+                                              c_vp]),
+    "rkv_ragged_append": (ctypes.c_int, [P(KVLayout), c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,
+                                         c_vp]),
+    "rkv_ragged_decode_attention_workspace_size": (c_sz, [P(Query), P(KVLayout)]),
+    "rkv_ragged_decode_attention": (ctypes.c_int, [P(Query), P(KVLayout), c_vp, c_vp, c_f32,
+                                                   P(Output), c_vp, c_vp, c_sz, c_vp]),
+    "rkv_ragged_error": (ctypes.c_int, [ctypes.c_int, P(c_i32)]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -165,7 +174,22 @@ DEVICE_ERRORS = {
     1: "a bounded wait inside a decode kernel gave up (the launch's output is incomplete)",
     2: "a page-table entry lies outside the page pool (that page was read as slot 0), or a "
        "batch reindex named a slot or a row outside the pool (that slot or row was left as it was)",
+    3: "a request's length lies outside its page table (it was read as the nearer bound)",
+    4: "a page-table step was refused: pages, slot-map entries or table columns were missing, or a "
+       "length or the free ring's state was out of range (no page was taken or given back)",
 }
+
+# Devices on which a ragged operator has run: their error words are read by check_device_errors.
+ragged_devices = set()
+
+
+def ragged_error(device_index: int, clear: bool = True) -> int:
+    """The ragged operators' error word of a device (waits for the device)."""
+    code = c_i32(0)
+    with torch.cuda.device(device_index):
+        check(load().rkv_ragged_error(1 if clear else 0, code), "rkv_ragged_error")
+    return code.value
+
 
 
 class DeviceError(RazorKVError):

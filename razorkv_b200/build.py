@@ -19,8 +19,9 @@ OBJ_DIR = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(HERE, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "librazorkv_b200.so")
 
-SOURCES = ["rkv_capi.cu", "rkv_generic.cu", "rkv_decode_sm100.cu", "rkv_noalloc.cu"]
-HEADERS = ["rkv_common.cuh", "rkv_kernels.h", "rkv_sm100.cuh"]
+SOURCES = ["rkv_capi.cu", "rkv_generic.cu", "rkv_decode_sm100.cu", "rkv_noalloc.cu",
+           "rkv_ragged.cu", "rkv_ragged_tables.cu", "rkv_ragged_decode.cu"]
+HEADERS = ["rkv_common.cuh", "rkv_kernels.h", "rkv_ragged.h", "rkv_sm100.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

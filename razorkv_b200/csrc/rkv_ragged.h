@@ -1,0 +1,51 @@
+// Parameter blocks and launchers of the ragged operators (requests of different lengths over
+// one page pool).  Internal to the library.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace rkv {
+namespace ragged {
+
+// Codes of the ragged kernels' error word (the same numbers as the Python DEVICE_ERRORS).
+constexpr int kErrPage = 2;      // a page or slot id outside the pool
+constexpr int kErrLength = 3;    // a length outside [0, table capacity]
+constexpr int kErrRefused = 4;   // a page-table step that could not be granted
+
+struct TableParams {
+    const int64_t* lengths; const int64_t* new_lengths; int64_t R, P;
+    int64_t* table; int64_t table_stride, W;
+    int64_t* ring; int64_t C; int64_t* state;
+    int64_t* out_lengths; int64_t* out_state;
+    int64_t* slot_map; int64_t* positions; int64_t M; int64_t* starts;
+};
+
+struct AppendParams {
+    void* k; void* v; int64_t stride_h, stride_p, stride_t, P, num_slots;
+    const void* k_new; const void* v_new; int64_t new_stride_t, new_stride_h;
+    int64_t T; const int64_t* slot_map; int Hkv, D, dtype;
+};
+
+struct DecodeParams {
+    const void* q; int64_t q_stride_b, q_stride_h;
+    const void* k; const void* v; int64_t stride_h, stride_p, stride_t, P, num_slots;
+    const int64_t* table; int64_t table_stride, W;
+    const int64_t* lengths; const int64_t* starts;
+    int B, Hq, Hkv, D, dtype;
+    float scale;
+    void* out; int64_t o_stride_b, o_stride_h; float* lse;
+    void* ws;
+};
+
+cudaError_t launch_tables(const TableParams& p, cudaStream_t st);
+cudaError_t launch_append(const AppendParams& p, cudaStream_t st);
+size_t decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st);
+
+// Reads (and with clear resets) the error word of one translation unit on the current device.
+cudaError_t read_table_error(int clear, int* code);
+cudaError_t read_decode_error(int clear, int* code);
+
+}  // namespace ragged
+}  // namespace rkv
