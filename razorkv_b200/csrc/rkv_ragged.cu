@@ -69,7 +69,7 @@ size_t rkv_ragged_decode_attention_workspace_size(const rkv_query* q, const rkv_
     if (!q || !pool || pool->num_kv_heads < 1 || pool->batch < 0 || pool->head_dim < 1 ||
         pool->head_dim > kMaxHeadDim || q->num_heads < 1 || q->num_heads % pool->num_kv_heads)
         return 0;
-    return ragged::decode_workspace_bytes(pool->batch, q->num_heads, pool->num_kv_heads, pool->head_dim);
+    return ragged::decode_workspace_bytes(q->num_heads, pool->num_kv_heads, pool->head_dim);
 }
 
 int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,

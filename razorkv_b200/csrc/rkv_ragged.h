@@ -40,7 +40,7 @@ struct DecodeParams {
 
 cudaError_t launch_tables(const TableParams& p, cudaStream_t st);
 cudaError_t launch_append(const AppendParams& p, cudaStream_t st);
-size_t decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+size_t decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D);
 cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st);
 
 // Reads (and with clear resets) the error word of one translation unit on the current device.
