@@ -102,6 +102,7 @@ int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
     p.scale = scale > 0.f ? scale : (float)(1.0 / sqrt((double)pool->head_dim));
     p.out = out->out; p.o_stride_b = out->stride_b; p.o_stride_h = out->stride_h; p.lse = lse;
     p.ws = workspace;
+    if (p.P < (1ll << 31)) p.div_p = ragged::FastDiv((uint32_t)p.P);
     return status_of(ragged::launch_decode(p, S(stream)));
 }
 

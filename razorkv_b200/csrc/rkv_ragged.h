@@ -13,6 +13,23 @@ constexpr int kErrPage = 2;      // a page or slot id outside the pool
 constexpr int kErrLength = 3;    // a length outside [0, table capacity]
 constexpr int kErrRefused = 4;   // a page-table step that could not be granted
 
+// Division of 31-bit numbers by a divisor known at launch: the multiplicative inverse rounded up,
+// 2^32 + mul = ceil(2^(32 + shift) / d) with 2^shift >= d, is exact below 2^31
+// (Granlund and Montgomery, "Division by invariant integers using multiplication").
+struct FastDiv {
+    uint32_t mul = 0; int shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d) {
+        while ((1ull << shift) < d) ++shift;
+        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        return (uint32_t)(((uint64_t)n * mul >> 32) + n >> shift);
+    }
+#endif
+};
+
 struct TableParams {
     const int64_t* lengths; const int64_t* new_lengths; int64_t R, P;
     int64_t* table; int64_t table_stride, W;
@@ -36,6 +53,7 @@ struct DecodeParams {
     float scale;
     void* out; int64_t o_stride_b, o_stride_h; float* lse;
     void* ws;
+    FastDiv div_p;      // by P, where it is below 2^31
 };
 
 cudaError_t launch_tables(const TableParams& p, cudaStream_t st);

@@ -30,6 +30,7 @@ namespace ragged {
 static __device__ int g_error;
 
 constexpr int kCtas = 148;      // one persistent CTA per SM
+constexpr int kMostWarps = 12;  // warps per CTA of any kernel here (16 at most: join_parts)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -52,19 +53,29 @@ __device__ __forceinline__ int64_t tiles_of(int64_t first, int64_t last) {
     return last > first ? (last + TT - 1) / TT - first / TT : 1;
 }
 
+// What a segment costs besides its tiles, in tiles: its queries, its outputs, the change of
+// pages.  Runs are of equal cost, so a segment of n tiles has n + kOver units, the first kOver of
+// which hold no tile.
+constexpr int kOver = 1;
+
+// a / b of non-negative numbers, the 32-bit way where it can be
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // n runs of as nearly equal length as may be, the longer ones first: with q = units / n and
 // x = units % n, run i starts at i q + min(i, x).
 struct Deal {
     int64_t q, x;
     __device__ __forceinline__ Deal(int64_t units, int64_t n) {
-        q = units < (1ll << 32) ? (int64_t)((uint32_t)units / (uint32_t)n) : units / n;
+        q = divide(units, n);
         x = units - q * n;
     }
     __device__ __forceinline__ int64_t start(int64_t i) const { return i * q + min(i, x); }
     // the run that holds a unit
     __device__ __forceinline__ int64_t of(int64_t unit) const {
         const int64_t longer = x * (q + 1);
-        return unit < longer ? unit / (q + 1) : x + (unit - longer) / q;
+        return unit < longer ? divide(unit, q + 1) : x + divide(unit - longer, q);
     }
 };
 
@@ -91,29 +102,29 @@ struct Workspace {
     __device__ Part warp(int64_t worker) const { return Part{base + (2 * kCtas + worker) * stride, HG, D}; }
 };
 
-// The runs of a CTA and of its warps.
+// The runs of a CTA and of a warp in it.
 struct Runs {
     int64_t total;          // units of all requests
-    int64_t ctas;           // CTAs that have a run (one unit per warp at least)
-    int64_t cta0, cta1;     // the CTA's run
-    int64_t unit;           // first unit of the warp's run
-    int64_t count;          // and its length
-    int b; int64_t u;       // request of that unit, and its place in it
+    int64_t ctas;           // CTAs that have a run (a unit per warp at least)
+    int64_t cta1;           // end of the CTA's run
+    int64_t count;          // tiles of the warp's run
+    int b, seg;             // its first tile: request, segment of the request, tile of the segment
+    int64_t tile, tiles, first, last;   // and the request's tiles per segment, and its tokens
 };
 
 template <int TT, int NW>
 __device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_tile) {
-    __shared__ int64_t warp_sums[NW];
-    __shared__ int s_b[NW];
-    __shared__ int64_t s_u[NW];
+    constexpr int T = NW * 32;
+    __shared__ int64_t s_sums[NW];
+    __shared__ int64_t s_before[T];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (p.B + NW * 32 - 1) / (NW * 32);
+    const int per = (p.B + T - 1) / T;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-    int64_t mine = 0;
+    int64_t mine = 0, f = 0, l = 0;
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-        int64_t f, l;
         range_of(p, b, &f, &l);
-        mine += tiles_of<TT>(f, l) * per_tile;
+        mine += (tiles_of<TT>(f, l) + kOver) * per_tile;
     }
     int64_t x = mine;
 #pragma unroll
@@ -121,174 +132,238 @@ __device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_til
         const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 31) warp_sums[warp] = x;
+    if (lane == 31) s_sums[warp] = x;
     __syncthreads();
     Runs r{};
     int64_t before = x - mine;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-        if (w < warp) before += warp_sums[w];
-        r.total += warp_sums[w];
+        const int64_t y = s_sums[w];
+        before += w < warp ? y : 0;
+        r.total += y;
     }
-    r.ctas = max((int64_t)1, min((int64_t)gridDim.x, r.total / NW));
+    s_before[tid] = before;
+    __syncthreads();
+    r.ctas = max((int64_t)1, min((int64_t)gridDim.x, divide(r.total, NW)));
     if (blockIdx.x >= r.ctas) return r;
     const Deal deal(r.total, r.ctas);
-    r.cta0 = deal.start(blockIdx.x);
+    const int64_t cta0 = deal.start(blockIdx.x);
     r.cta1 = deal.start(blockIdx.x + 1);
-    const Deal own(r.cta1 - r.cta0, NW);
-    r.unit = r.cta0 + own.start(warp);
-    r.count = r.cta0 + own.start(warp + 1) - r.unit;
-    // the threads whose requests hold the start of a warp's run walk them
-    if (mine > 0 && before < r.cta1 && before + mine > r.cta0) {
-        for (int w = 0; w < NW; ++w) {
-            const int64_t u = r.cta0 + own.start(w);
-            if (u < before || u >= before + mine) continue;
-            int64_t at = before;
-            for (int b = b0; b < b1; ++b) {
-                int64_t f, l;
-                range_of(p, b, &f, &l);
-                const int64_t k = tiles_of<TT>(f, l) * per_tile;
-                if (u < at + k) { s_b[w] = b; s_u[w] = u - at; break; }
-                at += k;
-            }
-        }
+    const Deal own(r.cta1 - cta0, NW);
+    // even lanes look for the start of the warp's run, odd ones for its end
+    const int64_t target = cta0 + own.start(warp + (lane & 1));
+    int i = 0;
+#pragma unroll
+    for (int step = 512; step > 0; step >>= 1)
+        if (i + step < T && s_before[i + step] <= target) i += step;
+    int64_t at = s_before[i];
+    int b = i * per;
+    int64_t units = 0;
+    if (b < p.B) {
+        range_of(p, b, &f, &l);
+        r.tiles = tiles_of<TT>(f, l);
+        units = (r.tiles + kOver) * per_tile;
     }
-    __syncthreads();
-    r.b = s_b[warp];
-    r.u = s_u[warp];
+#pragma unroll 1
+    for (int k = 1; k < per && b + 1 < p.B && target >= at + units; ++k) {
+        at += units;
+        ++b;
+        range_of(p, b, &f, &l);
+        r.tiles = tiles_of<TT>(f, l);
+        units = (r.tiles + kOver) * per_tile;
+    }
+    // tiles before the target: those of the requests before, and of this one
+    int64_t tiles_before;
+    if (target >= r.total) {
+        tiles_before = r.total - kOver * per_tile * p.B;
+    } else {
+        r.seg = (int)divide(target - at, r.tiles + kOver);
+        r.tile = max((int64_t)0, target - at - r.seg * (r.tiles + kOver) - kOver);
+        tiles_before = at - kOver * per_tile * b + r.seg * r.tiles + r.tile;
+    }
+    r.count = __shfl_sync(0xffffffffu, tiles_before, 1) - __shfl_sync(0xffffffffu, tiles_before, 0);
+    r.b = __shfl_sync(0xffffffffu, b, 0);
+    r.seg = __shfl_sync(0xffffffffu, r.seg, 0);
+    r.tile = __shfl_sync(0xffffffffu, r.tile, 0);
+    r.tiles = __shfl_sync(0xffffffffu, r.tiles, 0);
+    r.first = __shfl_sync(0xffffffffu, f, 0);
+    r.last = __shfl_sync(0xffffffffu, l, 0);
     return r;
 }
 
 // What a warp leaves for the join: the part of a segment that began before its run (`head`), and
-// of one that began in its run and goes on behind it (`tail`).  A part that is there at the end
-// of the run is in shared memory, a head that ended before is in the workspace.
+// of one that began in its run and goes on behind it (`tail`).  Of the warp's two places in shared
+// memory, a part that is there at the end of the run is in the first, and a head that ended
+// before (`early`) in the second.
 struct Left {
-    int head, ends, spilled, head_b, head_seg;
+    int head, ends, early, head_b, head_seg;
     int tail, tail_b, tail_seg;
-    int64_t rest;           // units of the last segment behind the run
+    int64_t rest;           // tiles of the last segment behind the run
 };
 
+__device__ __forceinline__ float4 lds_float4(uint32_t at, bool on) {
+    float4 v;
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
+                 "mov.f32 %1, 0f00000000;\n\tmov.f32 %2, 0f00000000;\n\tmov.f32 %3, 0f00000000;\n\t"
+                 "@q ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=&f"(v.x), "=&f"(v.y), "=&f"(v.z), "=&f"(v.w)
+                 : "r"(at), "r"((uint32_t)on)
+                 : "memory");
+    return v;
+}
+
 // Joins the parts of a CTA's warps.  In the order of the warps, a tail, or the first head, starts
-// a chain, the heads behind it belong to the same segment, and one that ends closes it.  For each
-// chain, a thread per row weighs the parts, then all threads add them up, VEC elements at a time.
-template <int NW, int HG, int VEC>
+// a chain, the heads behind it belong to the same segment, and one that ends closes it.  A warp
+// takes a row of a chain: lane v weighs the part of warp v, and the lanes add the row up, four
+// elements each.  parts: two places of `place` floats per warp, `stride` floats apart.
+template <int NW, int HG, int DT>
 __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r, const Workspace& ws,
-                                           const Left* left, float* parts, int64_t stride, int groups) {
-    __shared__ float s_weight[NW][HG], s_scale[HG];
+                                           const Left* left, float* parts, int stride, int place, int groups) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = p.Hq / p.Hkv;
     const int c = blockIdx.x;
+    const bool in = lane < NW;
+    const unsigned heads = __ballot_sync(0xffffffffu, in && left[lane].head);
+    const unsigned tails = __ballot_sync(0xffffffffu, in && left[lane].tail);
+    const unsigned closing = __ballot_sync(0xffffffffu, in && left[lane].head && left[lane].ends);
+    const unsigned early = __ballot_sync(0xffffffffu, in && left[lane].early);
     if (threadIdx.x == 0) ws.open[c] = make_int4(-1, 0, 0, 0);
-    for (int i = 0; i < NW + 1; ++i) {
-        // chain 0: the first head; chain w + 1: the tail of warp w
+    int turn = warp;    // rows are dealt to the warps over all chains
+    // chain 0: the first head; chain w + 1: the tail of warp w
+    unsigned todo = tails << 1 | (heads & 1);
+#pragma unroll 1
+    while (todo) {
+        const int i = __ffs(todo) - 1;
+        todo &= todo - 1;
         const int w = i == 0 ? 0 : i - 1;
-        if (i == 0 ? !left[0].head : !left[w].tail) continue;
-        int z = w;                      // last warp of the chain
-        bool closed = i == 0 && left[0].ends;
-        for (int v = w + 1; v < NW && !closed; ++v) {
-            if (!left[v].head) continue;    // an empty run
-            z = v;
-            closed = left[v].ends;
-        }
-        auto part = [&](int v) {
-            const bool spilled = left[v].spilled && !(i > 0 && v == w);
-            return spilled ? ws.warp((int64_t)c * NW + v) : Part{parts + v * stride, HG, p.D};
-        };
+        const unsigned behind = 0xfffffffeu << w;
+        const unsigned closers = i == 0 && (closing & 1) ? 1u : closing & behind;
+        const bool closed = closers != 0;
+        const unsigned upto = closed ? (closers & -closers) * 2 - 1 : 0xffffffffu;
+        const unsigned members = (heads & behind & upto) | 1u << w;
+        const unsigned second = i == 0 ? early : early & behind;
         const int b = i ? left[w].tail_b : left[w].head_b;
         const int seg = i ? left[w].tail_seg : left[w].head_seg;
-        const int hq0 = seg / groups * G + seg % groups * HG;
-        const int ng = min(HG, G - seg % groups * HG);
+        const int h = groups == 1 ? seg : seg / groups, gi = groups == 1 ? 0 : seg % groups;
+        const int hq0 = h * G + gi * HG, ng = min(HG, G - gi * HG);
         const bool whole = i > 0 && closed;
         const Part to = ws.cta(c, i > 0);
-        __syncthreads();    // the weights of the chain before
-        if (threadIdx.x < ng) {
-            const int row = threadIdx.x;
-            float top = -INFINITY;
-            for (int v = w; v <= z; ++v)
-                if (v == w || left[v].head) top = fmaxf(top, part(v).top(row));
-            const float base = top == -INFINITY ? 0.f : top;
-            float sum = 0.f;
-            for (int v = w; v <= z; ++v) {
-                if (v != w && !left[v].head) continue;
-                const Part from = part(v);
-                const float a = sm100::ex2(from.top(row) - base);
-                s_weight[v][row] = a;
-                sum += from.sum(row) * a;
-            }
-            s_scale[row] = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-            if (!whole) { to.top(row) = top; to.sum(row) = sum; }
-            else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + row] = top * kLn2 + logf(sum);
-        }
-        __syncthreads();
-        const int per_row = p.D / VEC;
-        for (int e = threadIdx.x; e < ng * per_row; e += NW * 32) {
-            const int row = e / per_row, d = (e - row * per_row) * VEC;
-            float o[VEC];
+        int row = turn;
+#pragma unroll 1
+        for (; row < ng; row += NW) {
+            const bool mine = members >> lane & 1;
+            const Part own{parts + (mine ? lane : w) * stride + (mine && second >> lane & 1 ? place : 0), HG, p.D};
+            const float t = mine ? own.top(row) : -INFINITY;
+            float top = t, sum = mine ? own.sum(row) : 0.f;
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) o[x] = 0.f;
-            for (int v = w; v <= z; ++v) {
-                if (v != w && !left[v].head) continue;
-                const float a = s_weight[v][row];
-                const float* from = part(v).acc(row) + d;
-                if constexpr (VEC == 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(from);
-                    o[0] += f.x * a; o[1] += f.y * a; o[2] += f.z * a; o[3] += f.w * a;
-                } else {
-                    o[0] += from[0] * a;
-                }
+            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float weight = mine ? sm100::ex2(t - (top == -INFINITY ? 0.f : top)) : 0.f;
+            if (mine) sum *= weight;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            top = __shfl_sync(0xffffffffu, top, 0);
+            sum = __shfl_sync(0xffffffffu, sum, 0);
+            const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            if (lane == 0) {
+                if (!whole) { to.top(row) = top; to.sum(row) = sum; }
+                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + row] = top * kLn2 + logf(sum);
             }
-            if (whole) {
+            const uint32_t from = sm100::smem_u32(parts + 2 * HG + row * p.D);
+#pragma unroll 1
+            for (int d = lane * 4; d - lane * 4 < p.D; d += 128) {
+                float o[4] = {0.f, 0.f, 0.f, 0.f};
+                const bool all = p.D % 4 == 0;
+                if (all) {
+#pragma unroll
+                    for (int v = 0; v < NW; ++v) {
+                        const float a = __shfl_sync(0xffffffffu, weight, v);
+                        const float4 f = lds_float4(from + (v * stride + (second >> v & 1 ? place : 0) + d) * 4,
+                                                    (members >> v & 1) && d < p.D);
+                        o[0] = fmaf(f.x, a, o[0]); o[1] = fmaf(f.y, a, o[1]);
+                        o[2] = fmaf(f.z, a, o[2]); o[3] = fmaf(f.w, a, o[3]);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int v = 0; v < NW; ++v) {
+                        const float a = __shfl_sync(0xffffffffu, weight, v);
+                        if (!(members >> v & 1)) continue;
+                        const float* f = parts + v * stride + (second >> v & 1 ? place : 0) + 2 * HG + row * p.D;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            if (d + x < p.D) o[x] = fmaf(f[d + x], a, o[x]);
+                    }
+                }
                 const int64_t at = (int64_t)b * p.o_stride_b + (int64_t)(hq0 + row) * p.o_stride_h + d;
 #pragma unroll
-                for (int x = 0; x < VEC; ++x) store_elt(p.out, at + x, p.dtype, o[x] * s_scale[row]);
-            } else {
-#pragma unroll
-                for (int x = 0; x < VEC; ++x) to.acc(row)[d + x] = o[x];
+                for (int x = 0; x < 4; ++x) {
+                    if (d + x >= p.D) break;
+                    if (whole) store_elt(p.out, at + x, DT < 0 ? p.dtype : DT, o[x] * scale);
+                    else to.acc(row)[d + x] = o[x];
+                }
             }
         }
+        turn = row - ng;
+        turn = turn >= NW ? turn - NW : turn;
         if (i > 0 && !closed && threadIdx.x == 0) {
+            const int z = 31 - __clz(members);      // last warp of the chain
             const int64_t last = r.cta1 + left[z].rest - 1;
             ws.open[c] = make_int4(b, seg, (int)(Deal(r.total, r.ctas).of(last) - c), 0);
         }
     }
 }
 
-// Position in the row of units: request, segment (kv head, group of query heads), tile.
+// Position in the row of tiles: request, kv head, group of query heads, tile.
 template <int TT>
 struct Walk {
-    int b, seg, tile, tiles, first, last;
-    __device__ __forceinline__ void enter(const DecodeParams& p, int request) {
+    int b, h, gi, tile, tiles, first, last;
+    __device__ __forceinline__ void start(const Runs& r, int groups) {
+        b = r.b;
+        h = groups == 1 ? r.seg : r.seg / groups;
+        gi = r.seg - h * groups;
+        tile = (int)r.tile;
+        tiles = (int)r.tiles;
+        first = (int)r.first;
+        last = (int)r.last;
+    }
+    __device__ __forceinline__ void next(const DecodeParams& p, int groups) {
+        if (++tile < tiles) return;
+        tile = 0;
+        if (++gi < groups) return;
+        gi = 0;
+        if (++h < p.Hkv) return;
+        h = 0;
+        if (++b >= p.B) return;
         int64_t f, l;
-        range_of(p, request, &f, &l);
-        b = request;
+        range_of(p, b, &f, &l);
         first = (int)f;
         last = (int)l;
         tiles = (int)tiles_of<TT>(f, l);
     }
-    __device__ __forceinline__ void next(const DecodeParams& p, int per_tile) {
-        if (++tile < tiles) return;
-        tile = 0;
-        if (++seg < per_tile) return;
-        seg = 0;
-        if (b + 1 < p.B) enter(p, b + 1);
-    }
-    __device__ __forceinline__ int token0() const { return (first / TT + tile) * TT; }
+    __device__ __forceinline__ int token0() const { return ((uint32_t)first / TT + tile) * TT; }
 };
 
 // ------------------------------------------------------------------------------------------
 // 16-bit types, on tensor cores.  One warp works alone: it copies its tiles (TT tokens of K and
 // V) into a ring of STAGES buffers of its own with 16-byte asynchronous copies, row by row
-// through the page table, and multiplies with m16n8k16 from there.
-//   S = Q K^T: the rows of A are query heads (MH of them), the columns of B are tokens;
-//   O = P V:   P stays in registers, since the accumulators of S have the layout of A.
+// through the page table, and multiplies with m16n8k16 from there, tokens and dims in the rows
+// and NH x 8 query heads in the columns:
+//   S^T = K Q^T  (16 tokens x 8 heads),    O^T += V^T P^T  (16 dims x 8 heads).
+// With the heads in the narrow dimension no product is spent on padding up to 16 rows, and O
+// takes half the registers.  P^T gets from the accumulator's layout to the operand's by an 8x8
+// transpose in registers.
 // Rounding P to 16 bits alone would add an error as large as the output's own rounding, so P
-// goes in as hi + lo, both 16-bit.  With up to 8 heads, rows 8..15 of A are free and hold lo:
-// the second half of the sum costs no instruction.  In fp16 the weights are scaled by 2^14
-// (kBias), so that small ones do not fall below fp16's range; the scale is part of the maximum
-// that is kept, and cancels.
+// goes in as hi + lo, both 16-bit.  The base of the power is a maximum seen so far that is
+// only renewed when a logit exceeds it by more than 2^kSlack, which saves the reduction over
+// lanes on most tiles; weights are then at most 2^kSlack instead of 1.  In fp16 they are scaled
+// by 2^kBias besides, so that small ones stay in fp16's normal range; that scale is part of the
+// base and cancels.
 // Rows outside the request's range are filled with zeros without being read: what the pool
 // holds there (NaN included) never enters a product.
 // ------------------------------------------------------------------------------------------
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0)
                  : "memory");
 }
@@ -320,221 +395,255 @@ struct TcShape {
     static constexpr int kSmem = NW * STAGES * kStage;
 };
 
-template <bool kBf16, int DP, int MH, int TT, int NW, int STAGES>
+constexpr float kSlack = 8.f;
+
+// kWhole: pages hold a multiple of 16 tokens, so 16 rows have one page.
+template <bool kBf16, int DP, int NH, int TT, int NW, int STAGES, bool kWhole>
 __global__ void __launch_bounds__(NW * 32, 1)
 decode_tc_kernel(DecodeParams p, int groups) {
     using Shape = TcShape<DP, TT, NW, STAGES>;
-    static_assert(TT % 16 == 0 && TT <= 32 && DP % 16 == 0 && (MH == 8 || MH == 16), "shape");
+    static_assert(TT % 16 == 0 && TT <= 32 && DP % 64 == 0 && (NH == 1 || NH == 2), "shape");
     extern __shared__ __align__(128) char smem[];
     __shared__ Left left[NW];
+    constexpr int MH = NH * 8;
     constexpr int kChunks = DP / 8;             // 16-byte chunks per row
-    constexpr int kCopies = TT * kChunks / 32;  // copies per lane for K, and for V
-    static_assert(TT * kChunks % 32 == 0, "a tile is a whole number of copies per lane");
-    static_assert(STAGES * Shape::kStage >= MH * (DP + 2) * 4, "a part fits the warp's ring");
-    constexpr float kBias = kBf16 ? 0.f : 14.f;
-    constexpr int kRows = MH / 8;               // heads per lane: g, and g + 8
-    constexpr int kQ = 2 * kRows;
+    constexpr int kCopies = 16 * kChunks / 32;  // copies per lane for 16 rows of K, and of V
+    static_assert(STAGES * Shape::kStage / 2 >= MH * (DP + 2) * 4 && STAGES * Shape::kStage % 32 == 0,
+                  "two parts fit the warp's ring");
+    constexpr float kBias = kBf16 ? 0.f : 6.f;
     // the next segment's queries are fetched a tile ahead where registers allow
-    constexpr bool kFetchQ = DP * MH <= 2048;
+    constexpr bool kFetchQ = DP * MH <= 1024;
     sm100::grid_launch_dependents();
     sm100::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per_tile = p.Hkv * groups;
     const int G = p.Hq / p.Hkv;
     const Workspace ws(p, MH);
 
-    const Runs runs = find_runs<TT, NW>(p, per_tile);
+    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
     }
     const uint32_t ring = sm100::smem_u32(smem) + warp * STAGES * Shape::kStage;
     const float scale2 = p.scale * kLog2e;
+    const float slack = kSlack / scale2;
     Left mine{};
+    // at the end of the run the ring is free and has room for two parts
+    float* places = reinterpret_cast<float*>(smem + warp * STAGES * Shape::kStage);
+    constexpr int kPlace = STAGES * Shape::kStage / 8;
     if (runs.count > 0) {
         const int count = (int)runs.count;
         Walk<TT> put, get, nx;
-        put.enter(p, runs.b);
-        put.seg = (int)(runs.u / put.tiles);
-        put.tile = (int)(runs.u % put.tiles);
+        put.start(runs, groups);
         get = put;
 
-        // ---- loads: lane r looks up row r of the tile; its page id is fetched a tile ahead
+        // ---- loads.  The lanes hold the ids of 32 pages in a row of the request, from page
+        // `win_at` on; lane r looks up row r of the tile there (kWhole: row 16 r, for 16 rows).
         int ahead = count;
-        const int P = (int)p.P;
-        auto fetch_page = [&]() -> int64_t {
-            const int t = put.token0() + lane;
-            return lane < TT && t >= put.first && t < put.last
-                       ? p.table[(int64_t)put.b * p.table_stride + t / P] : -1;
-        };
-        int64_t page = fetch_page();
+        const uint32_t P = (uint32_t)p.P;
+        int64_t window = 0;
+        uint32_t win_at = 0;
+        int win_b = -1;
         const char* kbytes = static_cast<const char*>(p.k);
-        const char* vbytes = static_cast<const char*>(p.v);
+        const int64_t v_from_k = static_cast<const char*>(p.v) - kbytes;
+        const int64_t row_bytes = p.stride_t * 2;
+        constexpr int kStep = 32 / kChunks > 0 ? 32 / kChunks : 1;     // rows between a lane's copies
+        const int lane_row = kChunks >= 32 ? 0 : lane / kChunks, lane_chunk = lane % kChunks;
+        const uint32_t lane_dst = lane_row * Shape::kPitch + lane_chunk * 16;
+        const int64_t lane_src = lane_row * row_bytes + lane_chunk * 16;
+        const bool in_row = lane_chunk * 8 < p.D;
         auto issue = [&](int stage) {
             if (ahead > 0) {
-                const int t = put.token0() + lane;
-                int64_t row = -1;
-                if (lane < TT && t >= put.first && t < put.last) {
-                    if (page < 0 || page >= p.num_slots) { atomicMax(&g_error, kErrPage); page = 0; }
-                    row = (page * p.stride_p + (int64_t)(t % P) * p.stride_t +
-                           (int64_t)(put.seg / groups) * p.stride_h) * 2;
+                const int t0 = put.token0();
+                const uint32_t p0 = p.div_p(max(t0, put.first));
+                const uint32_t p1 = p.div_p(max(min(t0 + TT, put.last) - 1, 0));
+                if (put.last > put.first && (put.b != win_b || p0 < win_at || p1 >= win_at + 32)) {
+                    win_b = put.b;
+                    win_at = p0;
+                    const int64_t at = (int64_t)p0 + lane;
+                    window = at * P < put.last ? p.table[(int64_t)put.b * p.table_stride + at] : 0;
+                    if (window < 0 || window >= p.num_slots) { atomicMax(&g_error, kErrPage); window = 0; }
                 }
-                const uint32_t dst = ring + stage * Shape::kStage;
+                const int tr = t0 + (kWhole ? lane * 16 : lane);
+                const uint32_t pr = p.div_p(tr);
+                const int64_t page = __shfl_sync(0xffffffffu, window, pr - win_at);
+                // byte offset of this lane's row (group of rows) in the pool
+                const int64_t row = (page * p.stride_p + (int64_t)((uint32_t)tr - pr * P) * p.stride_t +
+                                     (int64_t)put.h * p.stride_h) * 2;
+                const uint32_t dst = ring + stage * Shape::kStage + lane_dst;
+                if (kWhole && t0 >= put.first && t0 + TT <= put.last && p.D == DP) {
 #pragma unroll
-                for (int j = 0; j < kCopies; ++j) {
-                    const int i = lane + 32 * j, r = i / kChunks, c = i % kChunks;
-                    const int64_t off = __shfl_sync(0xffffffffu, row, r);
-                    const bool on = off >= 0 && c * 8 < p.D;
-                    const int64_t src = on ? off + c * 16 : 0;
-                    copy16(dst + r * Shape::kPitch + c * 16, kbytes + src, on);
-                    copy16(dst + Shape::kPlane + r * Shape::kPitch + c * 16, vbytes + src, on);
+                    for (int x = 0; x < TT / 16; ++x) {
+                        const char* src = kbytes + __shfl_sync(0xffffffffu, row, x) + lane_src;
+                        const uint32_t to = dst + x * 16 * Shape::kPitch;
+#pragma unroll
+                        for (int j = 0; j < kCopies; ++j) {
+                            copy16(to + j * kStep * Shape::kPitch, src);
+                            copy16(to + Shape::kPlane + j * kStep * Shape::kPitch, src + v_from_k);
+                            src += kStep * row_bytes;
+                        }
+                    }
+                } else {
+#pragma unroll 2
+                    for (int j = 0; j < kCopies * (TT / 16); ++j) {
+                        const int r = lane_row + j * kStep, t = t0 + r;
+                        int64_t off = __shfl_sync(0xffffffffu, row, kWhole ? r / 16 : r);
+                        const bool in = t >= put.first && t < put.last && in_row;
+                        if (kWhole) off += (int64_t)(r % 16) * row_bytes;
+                        const char* src = kbytes + (in ? off + lane_chunk * 16 : 0);
+                        copy16_or_zero(dst + j * kStep * Shape::kPitch, src, in);
+                        copy16_or_zero(dst + Shape::kPlane + j * kStep * Shape::kPitch, src + v_from_k, in);
+                    }
                 }
                 --ahead;
-                put.next(p, per_tile);
-                if (ahead > 0) page = fetch_page();
+                put.next(p, groups);
             }
             copies_commit();
         };
 
         // ---- products
         const int g = lane >> 2, c2 = (lane & 3) * 2;
-        uint32_t q[DP / 16][kQ], qn[kFetchQ ? DP / 16 : 1][kQ];
-        auto load_q = [&](const Walk<TT>& w, uint32_t (*to)[kQ]) {
-            const int g0 = (w.seg % groups) * MH, ng = min(MH, G - g0);
+        uint32_t q[DP / 16][NH][2], qn[kFetchQ ? DP / 16 : 1][NH][2];
+        auto load_q = [&](const Walk<TT>& w, uint32_t (*to)[NH][2]) {
+            const int g0 = w.gi * MH, ng = min(MH, G - g0);
             const char* qp = static_cast<const char*>(p.q) +
-                             ((int64_t)w.b * p.q_stride_b +
-                              (int64_t)(w.seg / groups * G + g0) * p.q_stride_h) * 2;
+                             ((int64_t)w.b * p.q_stride_b + (int64_t)(w.h * G + g0 + g) * p.q_stride_h + c2) * 2;
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
+            for (int n = 0; n < NH; ++n) {
+                const bool on = g + 8 * n < ng;
 #pragma unroll
-                for (int x = 0; x < kQ; ++x) {
-                    const int r = g + (x % kRows) * 8, d = k * 16 + c2 + x / kRows * 8;
-                    to[k][x] = r < ng && d < p.D
-                                   ? *reinterpret_cast<const uint32_t*>(qp + (r * p.q_stride_h + d) * 2) : 0u;
-                }
+                for (int k = 0; k < DP / 8; ++k)
+                    to[k / 2][n][k % 2] =
+                        on && k * 8 < p.D
+                            ? *reinterpret_cast<const uint32_t*>(qp + (8 * n * p.q_stride_h + k * 8) * 2) : 0u;
             }
         };
         load_q(get, q);
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) issue(s);
 
-        float o[DP / 8][4], m[kRows], l[kRows];
+        // column x of head block n: base of the power, the logit (unscaled) that renews it
+        // (-inf: none seen), and this lane's share of the sum
+        float o[DP / 16][NH][4], base[NH][2], limit[NH][2], l[NH][2];
         auto reset = [&]() {
 #pragma unroll
-            for (int n = 0; n < DP / 8; ++n)
+            for (int n = 0; n < NH; ++n) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
+                for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+                    for (int x = 0; x < 4; ++x) o[d][n][x] = 0.f;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) { base[n][x] = 0.f; limit[n][x] = -INFINITY; l[n][x] = 0.f; }
+            }
         };
         reset();
-        // ldmatrix rows of this lane: K (token, dim) as B, V (token, dim) transposed as B
-        const uint32_t k_lane = ((lane & 7) + (lane >> 4) * 8) * Shape::kPitch + ((lane >> 3) & 1) * 16;
-        const uint32_t v_lane = ((lane & 7) + ((lane >> 3) & 1) * 8) * Shape::kPitch + (lane >> 4) * 16;
+        // ldmatrix rows of this lane: K (token, dim) as A, V (token, dim) transposed as A
+        const uint32_t k_lane = ring + (lane & 15) * Shape::kPitch + (lane >> 4) * 16;
+        const uint32_t v_lane = ring + Shape::kPlane +
+                                ((lane & 7) + (lane >> 4) * 8) * Shape::kPitch + ((lane >> 3) & 1) * 16;
         int tile_in = get.tile;     // the segment's first tile in this run
         int stage = 0;
         for (int i = 0; i < count; ++i) {
             nx = get;
-            nx.next(p, per_tile);
+            nx.next(p, groups);
             if constexpr (kFetchQ)
-                if (i + 1 < count && nx.tile == 0) load_q(nx, qn);
+                if (nx.tile == 0 && i + 1 < count) load_q(nx, qn);
             copies_wait<STAGES - 1>();
             __syncwarp();
-            const uint32_t kt = ring + stage * Shape::kStage, vt = kt + Shape::kPlane;
-            float s[TT / 8][4];
+            const uint32_t kt = k_lane + stage * Shape::kStage, vt = v_lane + stage * Shape::kStage;
+            float s[TT / 16][NH][4];
 #pragma unroll
-            for (int n = 0; n < TT / 8; ++n)
+            for (int y = 0; y < TT / 16; ++y)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
+                for (int n = 0; n < NH; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[y][n][x] = 0.f;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
 #pragma unroll
-                for (int n = 0; n < TT / 16; ++n) {
-                    uint32_t b0, b1, b2, b3;
-                    sm100::ldsm_x4(kt + k_lane + n * 16 * Shape::kPitch + k * 32, b0, b1, b2, b3);
-                    if constexpr (MH == 16) {
-                        sm100::mma_16816<kBf16>(s[2 * n], q[k][0], q[k][1], q[k][2], q[k][3], b0, b1);
-                        sm100::mma_16816<kBf16>(s[2 * n + 1], q[k][0], q[k][1], q[k][2], q[k][3], b2, b3);
-                    } else {
-                        sm100::mma_16816<kBf16>(s[2 * n], q[k][0], 0u, q[k][1], 0u, b0, b1);
-                        sm100::mma_16816<kBf16>(s[2 * n + 1], q[k][0], 0u, q[k][1], 0u, b2, b3);
-                    }
+                for (int y = 0; y < TT / 16; ++y) {
+                    uint32_t a0, a1, a2, a3;
+                    sm100::ldsm_x4(kt + y * 16 * Shape::kPitch + k * 32, a0, a1, a2, a3);
+#pragma unroll
+                    for (int n = 0; n < NH; ++n)
+                        sm100::mma_16816<kBf16>(s[y][n], a0, a1, a2, a3, q[k][n][0], q[k][n][1]);
                 }
             }
             const int t0 = get.token0();
-            const bool edge = t0 < get.first || t0 + TT > get.last;
-            bool grew = false;
-            float alpha[kRows];
+            if (t0 < get.first || t0 + TT > get.last) {
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                float top = -INFINITY;
+                for (int y = 0; y < TT / 16; ++y) {
 #pragma unroll
-                for (int n = 0; n < TT / 8; ++n) {
+                    for (int x = 0; x < 4; ++x) {
+                        const int t = t0 + y * 16 + g + (x / 2) * 8;
+                        if (t < get.first || t >= get.last) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float v = s[n][2 * r + x] * scale2;
-                        if (edge) {
-                            const int t = t0 + n * 8 + c2 + x;
-                            if (t < get.first || t >= get.last) v = -INFINITY;
+                            for (int n = 0; n < NH; ++n) s[y][n][x] = -INFINITY;
                         }
-                        s[n][2 * r + x] = v;
-                        top = fmaxf(top, v);
                     }
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // a head without a finite logit so far keeps 0 as its base: 2^(-inf) = 0, no NaN
-                const float mn = fmaxf(m[r], top - kBias);
-                const float base = mn == -INFINITY ? 0.f : mn;
-                alpha[r] = sm100::ex2(m[r] - base);
-                grew = grew || mn > m[r];
-                m[r] = mn;
-                float sum = 0.f;
+            }
+            float top[NH][2];
+            bool over = false;
 #pragma unroll
-                for (int n = 0; n < TT / 8; ++n) {
+            for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float v = fmaxf(s[0][n][x], s[0][n][x + 2]);
+                    if constexpr (TT == 32) v = fmaxf(v, fmaxf(s[1][n][x], s[1][n][x + 2]));
+                    top[n][x] = v;
+                    over = over || v > limit[n][x];
+                }
+            }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float w = sm100::ex2(s[n][2 * r + x] - base);
-                        s[n][2 * r + x] = w;
-                        sum += w;
+                        float v = top[n][x];
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                        if (v > limit[n][x]) {
+                            const float b = v * scale2 - kBias;
+                            const float alpha = limit[n][x] == -INFINITY ? 0.f : sm100::ex2(base[n][x] - b);
+                            base[n][x] = b;
+                            limit[n][x] = v + slack;
+                            l[n][x] *= alpha;
+#pragma unroll
+                            for (int d = 0; d < DP / 16; ++d) {
+                                o[d][n][x] *= alpha;
+                                o[d][n][x + 2] *= alpha;
+                            }
+                        }
                     }
                 }
-                l[r] = l[r] * alpha[r] + sum;
-            }
-            if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n) {
-                    o[n][0] *= alpha[0];
-                    o[n][1] *= alpha[0];
-                    o[n][2] *= alpha[kRows - 1];
-                    o[n][3] *= alpha[kRows - 1];
-                }
             }
 #pragma unroll
-            for (int n = 0; n < TT / 16; ++n) {
-                uint32_t hi[2][kRows], lo[2][kRows];
+            for (int y = 0; y < TT / 16; ++y) {
+                uint32_t hi[NH][2], lo[NH][2];
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
+                for (int n = 0; n < NH; ++n) {
 #pragma unroll
-                    for (int r = 0; r < kRows; ++r) {
-                        const float w0 = s[2 * n + y][2 * r], w1 = s[2 * n + y][2 * r + 1];
-                        hi[y][r] = pack16<kBf16>(w0, w1);
-                        const float2 back = unpack16<kBf16>(hi[y][r]);
-                        lo[y][r] = pack16<kBf16>(w0 - back.x, w1 - back.y);
+                    for (int z = 0; z < 2; ++z) {   // tokens g, g + 8
+                        const float w0 = sm100::ex2(fmaf(s[y][n][2 * z], scale2, -base[n][0]));
+                        const float w1 = sm100::ex2(fmaf(s[y][n][2 * z + 1], scale2, -base[n][1]));
+                        l[n][0] += w0;
+                        l[n][1] += w1;
+                        const uint32_t h = pack16<kBf16>(w0, w1);
+                        const float2 back = unpack16<kBf16>(h);
+                        hi[n][z] = sm100::movmatrix_trans(h);
+                        lo[n][z] = sm100::movmatrix_trans(pack16<kBf16>(w0 - back.x, w1 - back.y));
                     }
                 }
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d) {
-                    uint32_t b0, b1, b2, b3;
-                    sm100::ldsm_x4_trans(vt + v_lane + n * 16 * Shape::kPitch + d * 32, b0, b1, b2, b3);
-                    if constexpr (MH == 16) {
-                        sm100::mma_16816<kBf16>(o[2 * d], hi[0][0], hi[0][1], hi[1][0], hi[1][1], b0, b1);
-                        sm100::mma_16816<kBf16>(o[2 * d + 1], hi[0][0], hi[0][1], hi[1][0], hi[1][1], b2, b3);
-                        sm100::mma_16816<kBf16>(o[2 * d], lo[0][0], lo[0][1], lo[1][0], lo[1][1], b0, b1);
-                        sm100::mma_16816<kBf16>(o[2 * d + 1], lo[0][0], lo[0][1], lo[1][0], lo[1][1], b2, b3);
-                    } else {
-                        sm100::mma_16816<kBf16>(o[2 * d], hi[0][0], lo[0][0], hi[1][0], lo[1][0], b0, b1);
-                        sm100::mma_16816<kBf16>(o[2 * d + 1], hi[0][0], lo[0][0], hi[1][0], lo[1][0], b2, b3);
+                    uint32_t a0, a1, a2, a3;
+                    sm100::ldsm_x4_trans(vt + y * 16 * Shape::kPitch + d * 32, a0, a1, a2, a3);
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        sm100::mma_16816<kBf16>(o[d][n], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                        sm100::mma_16816<kBf16>(o[d][n], a0, a1, a2, a3, lo[n][0], lo[n][1]);
                     }
                 }
             }
@@ -546,43 +655,65 @@ decode_tc_kernel(DecodeParams p, int groups) {
             const bool ends = get.tile + 1 == get.tiles, last = i + 1 == count;
             if (ends || last) {
                 const bool whole = tile_in == 0 && ends;
-                const int h = get.seg / groups, g0 = (get.seg % groups) * MH;
+                const int h = get.h, g0 = get.gi * MH;
                 const int ng = min(MH, G - g0);
                 if (!whole) {
                     if (tile_in > 0) {
-                        mine.head = 1; mine.ends = ends; mine.spilled = !last;
-                        mine.head_b = get.b; mine.head_seg = get.seg;
+                        mine.head = 1; mine.ends = ends; mine.early = !last;
+                        mine.head_b = get.b; mine.head_seg = h * groups + get.gi;
                     } else {
-                        mine.tail = 1; mine.tail_b = get.b; mine.tail_seg = get.seg;
+                        mine.tail = 1; mine.tail_b = get.b; mine.tail_seg = h * groups + get.gi;
                     }
                     mine.rest = get.tiles - get.tile - 1;
                 }
-                const Part part = last ? Part{reinterpret_cast<float*>(smem + warp * STAGES * Shape::kStage), MH, p.D}
+                const Part part = last ? Part{places, MH, p.D}
                                        : ws.warp((int64_t)blockIdx.x * NW + warp);
-                if (last) __syncwarp();
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) {
-                    float sum = l[r];
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    const int row = g + 8 * r;
-                    if (row >= ng) continue;
-                    const int hq = h * G + g0 + row;
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                    char* out = static_cast<char*>(p.out) +
-                                ((int64_t)get.b * p.o_stride_b + (int64_t)hq * p.o_stride_h) * 2;
+                for (int n = 0; n < NH; ++n) {
 #pragma unroll
-                    for (int n = 0; n < DP / 8; ++n) {
-                        const int d = n * 8 + c2;
-                        if (d >= p.D) break;
-                        const float x = MH == 16 ? o[n][2 * r] : o[n][0] + o[n][2];
-                        const float y = MH == 16 ? o[n][2 * r + 1] : o[n][1] + o[n][3];
-                        if (whole) *reinterpret_cast<uint32_t*>(out + d * 2) = pack16<kBf16>(x * inv, y * inv);
-                        else *reinterpret_cast<float2*>(part.acc(row) + d) = make_float2(x, y);
+                    for (int x = 0; x < 2; ++x) {
+                        float sum = l[n][x];
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                        const int row = 8 * n + c2 + x;
+                        const float b = limit[n][x] == -INFINITY ? -INFINITY : base[n][x];
+                        if (g == 0 && row < ng) {
+                            if (!whole) { part.top(row) = b; part.sum(row) = sum; }
+                            else if (p.lse) p.lse[(int64_t)get.b * p.Hq + h * G + g0 + row] = b * kLn2 + logf(sum);
+                        }
+                        if (whole) {
+                            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                            for (int d = 0; d < DP / 16; ++d) {
+                                o[d][n][x] *= inv;
+                                o[d][n][x + 2] *= inv;
+                            }
+                        } else if (row < ng) {
+                            float* acc = part.acc(row) + g;
+#pragma unroll
+                            for (int d = 0; d < DP / 16; ++d) {
+                                if (d * 16 < p.D) acc[d * 16] = o[d][n][x];
+                                if (d * 16 + 8 < p.D) acc[d * 16 + 8] = o[d][n][x + 2];
+                            }
+                        }
                     }
-                    if (c2 == 0) {
-                        if (!whole) { part.top(row) = m[r]; part.sum(row) = sum; }
-                        else if (p.lse) p.lse[(int64_t)get.b * p.Hq + hq] = m[r] * kLn2 + logf(sum);
+                    if (whole) {
+                        // dims in pairs, heads over the lanes
+                        const int row = 8 * n + g;
+                        char* out = static_cast<char*>(p.out) +
+                                    ((int64_t)get.b * p.o_stride_b +
+                                     (int64_t)(h * G + g0 + row) * p.o_stride_h + c2) * 2;
+#pragma unroll
+                        for (int d = 0; d < DP / 16; ++d) {
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) {
+                                const uint32_t v = sm100::movmatrix_trans(
+                                    pack16<kBf16>(o[d][n][2 * z], o[d][n][2 * z + 1]));
+                                if (row < ng && d * 16 + z * 8 < p.D)
+                                    *reinterpret_cast<uint32_t*>(out + (d * 16 + z * 8) * 2) = v;
+                            }
+                        }
                     }
                 }
                 reset();
@@ -592,7 +723,7 @@ decode_tc_kernel(DecodeParams p, int groups) {
 #pragma unroll
                         for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
-                            for (int x = 0; x < kQ; ++x) q[k][x] = qn[k][x];
+                            for (int n = 0; n < NH; ++n) { q[k][n][0] = qn[k][n][0]; q[k][n][1] = qn[k][n][1]; }
                     } else {
                         load_q(nx, q);
                     }
@@ -601,9 +732,16 @@ decode_tc_kernel(DecodeParams p, int groups) {
             get = nx;
         }
     }
+    if (mine.early) {   // a head that ended while the ring was in use comes back
+        __syncwarp();
+        const float4* from = reinterpret_cast<const float4*>(ws.warp((int64_t)blockIdx.x * NW + warp).at);
+        for (int i = lane; i < MH * (p.D + 2) / 4; i += 32)
+            reinterpret_cast<float4*>(places + kPlace)[i] = from[i];
+    }
     if (lane == 0) left[warp] = mine;
     __syncthreads();
-    join_parts<NW, MH, 4>(p, runs, ws, left, reinterpret_cast<float*>(smem), STAGES * Shape::kStage / 4, groups);
+    join_parts<NW, MH, kBf16 ? RKV_BF16 : RKV_F16>(p, runs, ws, left, reinterpret_cast<float*>(smem),
+                                                   2 * kPlace, kPlace, groups);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -614,15 +752,14 @@ constexpr int kAnyTile = 16, kAnyWarps = 8, kAnyHeads = 4;
 
 __global__ void __launch_bounds__(kAnyWarps * 32)
 decode_any_kernel(DecodeParams p, int groups) {
-    constexpr int HG = kAnyHeads;
+    constexpr int HG = kAnyHeads, kPlace = HG * (kMaxHeadDim + 2);
+    extern __shared__ __align__(128) char smem[];
     __shared__ Left left[kAnyWarps];
-    __shared__ float parts[kAnyWarps][HG * (kMaxHeadDim + 2)];
     sm100::grid_launch_dependents();
     sm100::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t per_tile = (int64_t)p.Hkv * groups;
     const Workspace ws(p, HG);
-    const Runs runs = find_runs<kAnyTile, kAnyWarps>(p, per_tile);
+    const Runs runs = find_runs<kAnyTile, kAnyWarps>(p, (int64_t)p.Hkv * groups);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
@@ -630,102 +767,104 @@ decode_any_kernel(DecodeParams p, int groups) {
     const int G = p.Hq / p.Hkv;
     const int ne = (p.D + 31) / 32;
     const float scale2 = p.scale * kLog2e;
+    float* places = reinterpret_cast<float*>(smem) + warp * 2 * kPlace;
     Left mine{};
-    int b = runs.b;
-    int64_t u = runs.u, todo = runs.count;
-    while (todo > 0) {
-        int64_t first, last;
-        range_of(p, b, &first, &last);
-        const int64_t tiles = tiles_of<kAnyTile>(first, last);
+    int b = runs.b, h = runs.seg / groups, gi = runs.seg % groups;
+    int64_t tile0 = runs.tile, tiles = runs.tiles, first = runs.first, last = runs.last;
+    for (int64_t todo = runs.count; todo > 0;) {
+        const int64_t tile1 = min(tiles, tile0 + todo);
         const int64_t* table = p.table + (int64_t)b * p.table_stride;
-        while (todo > 0 && u < tiles * per_tile) {
-            const int64_t seg = u / tiles, tile0 = u - seg * tiles;
-            const int64_t tile1 = min(tiles, tile0 + todo);
-            const int h = (int)(seg / groups), g0 = (int)(seg % groups) * HG;
-            const int ng = min(HG, G - g0);
-            const int64_t q0 = (int64_t)b * p.q_stride_b + (int64_t)(h * G + g0) * p.q_stride_h;
-            float q[HG][8], acc[HG][8], m[HG], l[HG];
+        const int g0 = gi * HG, ng = min(HG, G - g0);
+        const int64_t q0 = (int64_t)b * p.q_stride_b + (int64_t)(h * G + g0) * p.q_stride_h;
+        float q[HG][8], acc[HG][8], m[HG], l[HG];
+#pragma unroll
+        for (int g = 0; g < HG; ++g) {
+            m[g] = -INFINITY;
+            l[g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = lane + 32 * i;
+                q[g][i] = g < ng && e < p.D ? load_elt(p.q, q0 + g * p.q_stride_h + e, p.dtype) : 0.f;
+                acc[g][i] = 0.f;
+            }
+        }
+        const int64_t t1 = min(last, (first / kAnyTile + tile1) * kAnyTile);
+        for (int64_t t = max(first, (first / kAnyTile + tile0) * kAnyTile); t < t1; ++t) {
+            const int64_t j = t / p.P;
+            int64_t page = table[j];
+            if (page < 0 || page >= p.num_slots) { atomicMax(&g_error, kErrPage); page = 0; }
+            const int64_t off = page * p.stride_p + (t - j * p.P) * p.stride_t + (int64_t)h * p.stride_h;
+            float kr[8], vr[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = lane + 32 * i;
+                kr[i] = i < ne && e < p.D ? load_elt(p.k, off + e, p.dtype) : 0.f;
+                vr[i] = i < ne && e < p.D ? load_elt(p.v, off + e, p.dtype) : 0.f;
+            }
 #pragma unroll
             for (int g = 0; g < HG; ++g) {
-                m[g] = -INFINITY;
-                l[g] = 0.f;
+                float s = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = lane + 32 * i;
-                    q[g][i] = g < ng && e < p.D ? load_elt(p.q, q0 + g * p.q_stride_h + e, p.dtype) : 0.f;
-                    acc[g][i] = 0.f;
-                }
+                for (int i = 0; i < 8; ++i) s = fmaf(q[g][i], kr[i], s);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                s *= scale2;
+                const float mn = fmaxf(m[g], s);
+                const float base = mn == -INFINITY ? 0.f : mn;
+                const float alpha = sm100::ex2(m[g] - base), w = sm100::ex2(s - base);
+                m[g] = mn;
+                l[g] = l[g] * alpha + w;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[g][i] = acc[g][i] * alpha + w * vr[i];
             }
-            const int64_t t1 = min(last, (first / kAnyTile + tile1) * kAnyTile);
-            for (int64_t t = max(first, (first / kAnyTile + tile0) * kAnyTile); t < t1; ++t) {
-                const int64_t j = t / p.P;
-                int64_t page = table[j];
-                if (page < 0 || page >= p.num_slots) { atomicMax(&g_error, kErrPage); page = 0; }
-                const int64_t off = page * p.stride_p + (t - j * p.P) * p.stride_t + (int64_t)h * p.stride_h;
-                float kr[8], vr[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = lane + 32 * i;
-                    kr[i] = i < ne && e < p.D ? load_elt(p.k, off + e, p.dtype) : 0.f;
-                    vr[i] = i < ne && e < p.D ? load_elt(p.v, off + e, p.dtype) : 0.f;
-                }
-#pragma unroll
-                for (int g = 0; g < HG; ++g) {
-                    float s = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) s = fmaf(q[g][i], kr[i], s);
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                    s *= scale2;
-                    const float mn = fmaxf(m[g], s);
-                    const float base = mn == -INFINITY ? 0.f : mn;
-                    const float alpha = sm100::ex2(m[g] - base), w = sm100::ex2(s - base);
-                    m[g] = mn;
-                    l[g] = l[g] * alpha + w;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[g][i] = acc[g][i] * alpha + w * vr[i];
-                }
+        }
+        todo -= tile1 - tile0;
+        const bool ends = tile1 == tiles, whole = tile0 == 0 && ends;
+        const bool is_early = !whole && tile0 > 0 && todo > 0;
+        if (!whole) {
+            if (tile0 > 0) {
+                mine.head = 1; mine.ends = ends; mine.early = is_early;
+                mine.head_b = b; mine.head_seg = h * groups + gi;
+            } else {
+                mine.tail = 1; mine.tail_b = b; mine.tail_seg = h * groups + gi;
             }
-            todo -= tile1 - tile0;
-            u += tile1 - tile0;
-            const bool ends = tile1 == tiles, whole = tile0 == 0 && ends;
-            if (!whole) {
-                if (tile0 > 0) {
-                    mine.head = 1; mine.ends = ends; mine.spilled = todo > 0;
-                    mine.head_b = b; mine.head_seg = (int)seg;
-                } else {
-                    mine.tail = 1; mine.tail_b = b; mine.tail_seg = (int)seg;
-                }
-                mine.rest = tiles - tile1;
+            mine.rest = tiles - tile1;
+        }
+        const Part part{places + (is_early ? kPlace : 0), HG, p.D};
+#pragma unroll
+        for (int g = 0; g < HG; ++g) {
+            if (g >= ng) break;
+            const int hq = h * G + g0 + g;
+            const float inv = l[g] == 0.f ? 0.f : 1.f / l[g];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = lane + 32 * i;
+                if (e >= p.D) break;
+                if (whole)
+                    store_elt(p.out, (int64_t)b * p.o_stride_b + (int64_t)hq * p.o_stride_h + e,
+                              p.dtype, acc[g][i] * inv);
+                else part.acc(g)[e] = acc[g][i];
             }
-            const Part part = todo == 0 ? Part{parts[warp], HG, p.D}
-                                        : ws.warp((int64_t)blockIdx.x * kAnyWarps + warp);
-#pragma unroll
-            for (int g = 0; g < HG; ++g) {
-                if (g >= ng) break;
-                const int hq = h * G + g0 + g;
-                const float inv = l[g] == 0.f ? 0.f : 1.f / l[g];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = lane + 32 * i;
-                    if (e >= p.D) break;
-                    if (whole)
-                        store_elt(p.out, (int64_t)b * p.o_stride_b + (int64_t)hq * p.o_stride_h + e,
-                                  p.dtype, acc[g][i] * inv);
-                    else part.acc(g)[e] = acc[g][i];
-                }
-                if (lane == 0) {
-                    if (!whole) { part.top(g) = m[g]; part.sum(g) = l[g]; }
-                    else if (p.lse) p.lse[(int64_t)b * p.Hq + hq] = m[g] * kLn2 + logf(l[g]);
+            if (lane == 0) {
+                if (!whole) { part.top(g) = m[g]; part.sum(g) = l[g]; }
+                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq] = m[g] * kLn2 + logf(l[g]);
+            }
+        }
+        tile0 = 0;
+        if (++gi == groups) {
+            gi = 0;
+            if (++h == p.Hkv) {
+                h = 0;
+                if (++b < p.B) {
+                    range_of(p, b, &first, &last);
+                    tiles = tiles_of<kAnyTile>(first, last);
                 }
             }
         }
-        ++b;
-        u = 0;
     }
     if (lane == 0) left[warp] = mine;
     __syncthreads();
-    join_parts<kAnyWarps, kAnyHeads, 1>(p, runs, ws, left, parts[0], HG * (kMaxHeadDim + 2), groups);
+    join_parts<kAnyWarps, HG, -1>(p, runs, ws, left, reinterpret_cast<float*>(smem), 2 * kPlace, kPlace, groups);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -830,35 +969,40 @@ cudaError_t launch_pair(Kernel kernel, int threads, int smem, const DecodeParams
     return counted(cudaLaunchKernelEx(&cfg, merge_kernel, p, groups, HG), 1);
 }
 
-template <bool kBf16, int DP, int MH>
+template <bool kBf16, int DP, int NH, bool kWhole>
 cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
-    constexpr int TT = DP <= 64 ? 32 : 16, NW = 8, STAGES = DP <= 128 ? 3 : 2 - (DP > 192);
+    constexpr int TT = DP <= 64 ? 32 : 16, NW = DP <= 128 ? 12 : 6, STAGES = 2;
     using Shape = TcShape<DP, TT, NW, STAGES>;
-    static_assert(Shape::kSmem <= 232448 - 2048, "shared memory");
-    return launch_pair(decode_tc_kernel<kBf16, DP, MH, TT, NW, STAGES>, NW * 32, Shape::kSmem, p, MH, st);
+    static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 3072, "shared memory");
+    return launch_pair(decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>, NW * 32, Shape::kSmem, p,
+                       NH * 8, st);
+}
+
+template <int DP, int NH>
+cudaError_t launch_tc_dim(const DecodeParams& p, cudaStream_t st) {
+    const bool whole = p.P % 16 == 0;
+    if (p.dtype == RKV_BF16) return whole ? launch_tc<true, DP, NH, true>(p, st) : launch_tc<true, DP, NH, false>(p, st);
+    return whole ? launch_tc<false, DP, NH, true>(p, st) : launch_tc<false, DP, NH, false>(p, st);
 }
 
 template <int DP>
-cudaError_t launch_tc_dim(const DecodeParams& p, cudaStream_t st) {
-    const bool wide = p.Hq / p.Hkv > 8;
-    if (p.dtype == RKV_BF16) return wide ? launch_tc<true, DP, 16>(p, st) : launch_tc<true, DP, 8>(p, st);
-    return wide ? launch_tc<false, DP, 16>(p, st) : launch_tc<false, DP, 8>(p, st);
+cudaError_t launch_tc_heads(const DecodeParams& p, cudaStream_t st) {
+    return p.Hq / p.Hkv > 8 ? launch_tc_dim<DP, 2>(p, st) : launch_tc_dim<DP, 1>(p, st);
 }
 
 }  // namespace
 
 // Upper bound over the kernels that a call of these sizes may take.
 size_t decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D) {
-    return Workspace::bytes(8, Hq / Hkv > 8 ? 16 : 8, D);
+    return Workspace::bytes(kMostWarps, Hq / Hkv > 8 ? 16 : 8, D);
 }
 
 cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
-    if (!tc_ok(p)) return launch_pair(decode_any_kernel, kAnyWarps * 32, 0, p, kAnyHeads, st);
-    if (p.D <= 64) return launch_tc_dim<64>(p, st);
-    if (p.D <= 96) return launch_tc_dim<96>(p, st);
-    if (p.D <= 128) return launch_tc_dim<128>(p, st);
-    if (p.D <= 192) return launch_tc_dim<192>(p, st);
-    return launch_tc_dim<256>(p, st);
+    if (!tc_ok(p)) return launch_pair(decode_any_kernel, kAnyWarps * 32,
+                                       kAnyWarps * 2 * kAnyHeads * (kMaxHeadDim + 2) * (int)sizeof(float), p, kAnyHeads, st);
+    if (p.D <= 64) return launch_tc_heads<64>(p, st);
+    if (p.D <= 128) return launch_tc_heads<128>(p, st);
+    return launch_tc_heads<256>(p, st);
 }
 
 cudaError_t read_decode_error(int clear, int* code) {
