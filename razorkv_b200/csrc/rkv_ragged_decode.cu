@@ -34,6 +34,10 @@ constexpr int kMostWarps = 12;  // warps per CTA of any kernel here (16 at most:
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Natural logarithm of sum * 2^top.  The hardware's log2 is off by at most 2^-22 (absolutely, or
+// relatively to a result above one), as much as the hardware's 2^x in the sum itself.
+__device__ __forceinline__ float lse_of(float top, float sum) { return (top + __log2f(sum)) * kLn2; }
+
 // First and last token of request b, clamped to the page table's capacity.
 __device__ __forceinline__ void range_of(const DecodeParams& p, int b, int64_t* first, int64_t* last) {
     const int64_t capacity = p.W * p.P;
@@ -79,12 +83,15 @@ struct Deal {
     }
 };
 
-// A part of a segment in memory: HG x {maximum, sum}, then HG x D accumulators.
+// A part of a segment in memory: HG x {maximum, sum}, then HG rows of D accumulators, D + 4
+// floats apart (in shared memory, the 8 rows x 4 columns that a warp writes at a time then lie
+// in different banks).
 struct Part {
     float* at; int HG, D;
     __device__ float& top(int row) const { return at[2 * row]; }
     __device__ float& sum(int row) const { return at[2 * row + 1]; }
-    __device__ float* acc(int row) const { return at + 2 * HG + row * D; }
+    __device__ float* acc(int row) const { return at + 2 * HG + row * (D + 4); }
+    __host__ __device__ static constexpr int floats(int hg, int d) { return hg * (d + 6); }
 };
 
 // Workspace: for each CTA what the part at the end of its run belongs to, then two parts per
@@ -93,11 +100,11 @@ struct Part {
 struct Workspace {
     int4* open; float* base; int64_t stride; int HG, D;
     __host__ __device__ static int64_t bytes(int64_t warps, int64_t HG, int64_t D) {
-        return kCtas * 16 + (2 * kCtas + kCtas * warps) * HG * (D + 2) * 4;
+        return kCtas * 16 + (2 + warps) * kCtas * Part::floats((int)HG, (int)D) * 4;
     }
     __device__ Workspace(const DecodeParams& p, int hg)
         : open(static_cast<int4*>(p.ws)), base(reinterpret_cast<float*>(open + kCtas)),
-          stride((int64_t)hg * (p.D + 2)), HG(hg), D(p.D) {}
+          stride(Part::floats(hg, p.D)), HG(hg), D(p.D) {}
     __device__ Part cta(int c, int which) const { return Part{base + (2 * c + which) * stride, HG, D}; }
     __device__ Part warp(int64_t worker) const { return Part{base + (2 * kCtas + worker) * stride, HG, D}; }
 };
@@ -266,9 +273,9 @@ __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r,
             const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
             if (lane == 0) {
                 if (!whole) { to.top(row) = top; to.sum(row) = sum; }
-                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + row] = top * kLn2 + logf(sum);
+                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + row] = lse_of(top, sum);
             }
-            const uint32_t from = sm100::smem_u32(parts + 2 * HG + row * p.D);
+            const uint32_t from = sm100::smem_u32(Part{parts, HG, p.D}.acc(row));
 #pragma unroll 1
             for (int d = lane * 4; d - lane * 4 < p.D; d += 128) {
                 float o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -287,7 +294,7 @@ __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r,
                     for (int v = 0; v < NW; ++v) {
                         const float a = __shfl_sync(0xffffffffu, weight, v);
                         if (!(members >> v & 1)) continue;
-                        const float* f = parts + v * stride + (second >> v & 1 ? place : 0) + 2 * HG + row * p.D;
+                        const float* f = Part{parts + v * stride + (second >> v & 1 ? place : 0), HG, p.D}.acc(row);
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
                             if (d + x < p.D) o[x] = fmaf(f[d + x], a, o[x]);
@@ -360,9 +367,7 @@ struct Walk {
 // Rows outside the request's range are filled with zeros without being read: what the pool
 // holds there (NaN included) never enters a product.
 // ------------------------------------------------------------------------------------------
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
+// 16 bytes, or zeros without a read
 __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0)
                  : "memory");
@@ -387,11 +392,11 @@ __device__ __forceinline__ float2 unpack16(uint32_t x) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-template <int DP, int TT, int NW, int STAGES>
+template <int DP, int NH, int TT, int NW, int STAGES>
 struct TcShape {
     static constexpr int kPitch = DP * 2 + 16;          // odd in 16-byte units: no bank conflicts
     static constexpr int kPlane = TT * kPitch;          // K or V of a tile
-    static constexpr int kStage = 2 * kPlane;
+    static constexpr int kStage = 2 * kPlane + NH * 8 * kPitch;     // and the queries of its segment
     static constexpr int kSmem = NW * STAGES * kStage;
 };
 
@@ -401,18 +406,16 @@ constexpr float kSlack = 8.f;
 template <bool kBf16, int DP, int NH, int TT, int NW, int STAGES, bool kWhole>
 __global__ void __launch_bounds__(NW * 32, 1)
 decode_tc_kernel(DecodeParams p, int groups) {
-    using Shape = TcShape<DP, TT, NW, STAGES>;
+    using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(TT % 16 == 0 && TT <= 32 && DP % 64 == 0 && (NH == 1 || NH == 2), "shape");
     extern __shared__ __align__(128) char smem[];
     __shared__ Left left[NW];
     constexpr int MH = NH * 8;
     constexpr int kChunks = DP / 8;             // 16-byte chunks per row
     constexpr int kCopies = 16 * kChunks / 32;  // copies per lane for 16 rows of K, and of V
-    static_assert(STAGES * Shape::kStage / 2 >= MH * (DP + 2) * 4 && STAGES * Shape::kStage % 32 == 0,
+    static_assert(STAGES * Shape::kStage / 2 >= Part::floats(MH, DP) * 4 && STAGES * Shape::kStage % 32 == 0,
                   "two parts fit the warp's ring");
     constexpr float kBias = kBf16 ? 0.f : 6.f;
-    // the next segment's queries are fetched a tile ahead where registers allow
-    constexpr bool kFetchQ = DP * MH <= 1024;
     sm100::grid_launch_dependents();
     sm100::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -433,7 +436,7 @@ decode_tc_kernel(DecodeParams p, int groups) {
     constexpr int kPlace = STAGES * Shape::kStage / 8;
     if (runs.count > 0) {
         const int count = (int)runs.count;
-        Walk<TT> put, get, nx;
+        Walk<TT> put, get;
         put.start(runs, groups);
         get = put;
 
@@ -452,9 +455,24 @@ decode_tc_kernel(DecodeParams p, int groups) {
         const uint32_t lane_dst = lane_row * Shape::kPitch + lane_chunk * 16;
         const int64_t lane_src = lane_row * row_bytes + lane_chunk * 16;
         const bool in_row = lane_chunk * 8 < p.D;
+        // A segment's queries come with the first of its tiles in the run: a load of their own would
+        // stand behind the copies that are under way.
+        bool with_q = true;
         auto issue = [&](int stage) {
             if (ahead > 0) {
                 const int t0 = put.token0();
+                if (with_q) {
+                    const int g0 = put.gi * MH, ng = min(MH, G - g0);
+                    const char* src = static_cast<const char*>(p.q) +
+                                      ((int64_t)put.b * p.q_stride_b + (int64_t)(put.h * G + g0) * p.q_stride_h) * 2;
+                    const uint32_t to = ring + stage * Shape::kStage + 2 * Shape::kPlane;
+#pragma unroll
+                    for (int j = 0; j < MH * kChunks / 32; ++j) {
+                        const int i = lane + 32 * j, r = i / kChunks, c = i % kChunks;
+                        copy16_or_zero(to + r * Shape::kPitch + c * 16, src + r * p.q_stride_h * 2 + c * 16,
+                                       r < ng && c * 8 < p.D);
+                    }
+                }
                 const uint32_t p0 = p.div_p(max(t0, put.first));
                 const uint32_t p1 = p.div_p(max(min(t0 + TT, put.last) - 1, 0));
                 if (put.last > put.first && (put.b != win_b || p0 < win_at || p1 >= win_at + 32)) {
@@ -471,54 +489,41 @@ decode_tc_kernel(DecodeParams p, int groups) {
                 const int64_t row = (page * p.stride_p + (int64_t)((uint32_t)tr - pr * P) * p.stride_t +
                                      (int64_t)put.h * p.stride_h) * 2;
                 const uint32_t dst = ring + stage * Shape::kStage + lane_dst;
-                if (kWhole && t0 >= put.first && t0 + TT <= put.last && p.D == DP) {
+                // rows of the tile that this lane's copies read: [lo, lo + n), counted from its first
+                const int lo = put.first - t0 - lane_row;
+                const uint32_t n = in_row ? max(put.last - put.first, 0) : 0;
+                if (kWhole) {
 #pragma unroll
                     for (int x = 0; x < TT / 16; ++x) {
                         const char* src = kbytes + __shfl_sync(0xffffffffu, row, x) + lane_src;
                         const uint32_t to = dst + x * 16 * Shape::kPitch;
 #pragma unroll
                         for (int j = 0; j < kCopies; ++j) {
-                            copy16(to + j * kStep * Shape::kPitch, src);
-                            copy16(to + Shape::kPlane + j * kStep * Shape::kPitch, src + v_from_k);
+                            const bool on = (uint32_t)(x * 16 + j * kStep - lo) < n;
+                            copy16_or_zero(to + j * kStep * Shape::kPitch, src, on);
+                            copy16_or_zero(to + Shape::kPlane + j * kStep * Shape::kPitch, src + v_from_k, on);
                             src += kStep * row_bytes;
                         }
                     }
                 } else {
-#pragma unroll 2
+#pragma unroll
                     for (int j = 0; j < kCopies * (TT / 16); ++j) {
-                        const int r = lane_row + j * kStep, t = t0 + r;
-                        int64_t off = __shfl_sync(0xffffffffu, row, kWhole ? r / 16 : r);
-                        const bool in = t >= put.first && t < put.last && in_row;
-                        if (kWhole) off += (int64_t)(r % 16) * row_bytes;
-                        const char* src = kbytes + (in ? off + lane_chunk * 16 : 0);
-                        copy16_or_zero(dst + j * kStep * Shape::kPitch, src, in);
-                        copy16_or_zero(dst + Shape::kPlane + j * kStep * Shape::kPitch, src + v_from_k, in);
+                        const bool on = (uint32_t)(j * kStep - lo) < n;
+                        const char* src = kbytes + __shfl_sync(0xffffffffu, row, lane_row + j * kStep) + lane_chunk * 16;
+                        copy16_or_zero(dst + j * kStep * Shape::kPitch, src, on);
+                        copy16_or_zero(dst + Shape::kPlane + j * kStep * Shape::kPitch, src + v_from_k, on);
                     }
                 }
                 --ahead;
                 put.next(p, groups);
+                with_q = put.tile == 0;
             }
             copies_commit();
         };
 
         // ---- products
         const int g = lane >> 2, c2 = (lane & 3) * 2;
-        uint32_t q[DP / 16][NH][2], qn[kFetchQ ? DP / 16 : 1][NH][2];
-        auto load_q = [&](const Walk<TT>& w, uint32_t (*to)[NH][2]) {
-            const int g0 = w.gi * MH, ng = min(MH, G - g0);
-            const char* qp = static_cast<const char*>(p.q) +
-                             ((int64_t)w.b * p.q_stride_b + (int64_t)(w.h * G + g0 + g) * p.q_stride_h + c2) * 2;
-#pragma unroll
-            for (int n = 0; n < NH; ++n) {
-                const bool on = g + 8 * n < ng;
-#pragma unroll
-                for (int k = 0; k < DP / 8; ++k)
-                    to[k / 2][n][k % 2] =
-                        on && k * 8 < p.D
-                            ? *reinterpret_cast<const uint32_t*>(qp + (8 * n * p.q_stride_h + k * 8) * 2) : 0u;
-            }
-        };
-        load_q(get, q);
+        uint32_t q[DP / 16][NH][2];
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) issue(s);
 
@@ -537,19 +542,25 @@ decode_tc_kernel(DecodeParams p, int groups) {
             }
         };
         reset();
-        // ldmatrix rows of this lane: K (token, dim) as A, V (token, dim) transposed as A
+        // ldmatrix rows of this lane: K (token, dim) as A, V (token, dim) transposed as A, and
+        // queries (head, dim) as B
+        const uint32_t q_lane = ring + 2 * Shape::kPlane + (lane & 7) * Shape::kPitch + (lane >> 3) * 16;
         const uint32_t k_lane = ring + (lane & 15) * Shape::kPitch + (lane >> 4) * 16;
         const uint32_t v_lane = ring + Shape::kPlane +
                                 ((lane & 7) + (lane >> 4) * 8) * Shape::kPitch + ((lane >> 3) & 1) * 16;
         int tile_in = get.tile;     // the segment's first tile in this run
         int stage = 0;
         for (int i = 0; i < count; ++i) {
-            nx = get;
-            nx.next(p, groups);
-            if constexpr (kFetchQ)
-                if (nx.tile == 0 && i + 1 < count) load_q(nx, qn);
             copies_wait<STAGES - 1>();
             __syncwarp();
+            if (get.tile == tile_in) {
+#pragma unroll
+                for (int n = 0; n < NH; ++n)
+#pragma unroll
+                    for (int k = 0; k < DP / 32; ++k)
+                        sm100::ldsm_x4(q_lane + stage * Shape::kStage + n * 8 * Shape::kPitch + k * 64,
+                                       q[2 * k][n][0], q[2 * k][n][1], q[2 * k + 1][n][0], q[2 * k + 1][n][1]);
+            }
             const uint32_t kt = k_lane + stage * Shape::kStage, vt = v_lane + stage * Shape::kStage;
             float s[TT / 16][NH][4];
 #pragma unroll
@@ -604,17 +615,16 @@ decode_tc_kernel(DecodeParams p, int groups) {
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                        if (v > limit[n][x]) {
-                            const float b = v * scale2 - kBias;
-                            const float alpha = limit[n][x] == -INFINITY ? 0.f : sm100::ex2(base[n][x] - b);
-                            base[n][x] = b;
-                            limit[n][x] = v + slack;
-                            l[n][x] *= alpha;
+                        const bool renew = v > limit[n][x];
+                        const float b = v * scale2 - kBias;
+                        const float alpha = !renew ? 1.f : limit[n][x] == -INFINITY ? 0.f : sm100::ex2(base[n][x] - b);
+                        base[n][x] = renew ? b : base[n][x];
+                        limit[n][x] = renew ? v + slack : limit[n][x];
+                        l[n][x] *= alpha;
 #pragma unroll
-                            for (int d = 0; d < DP / 16; ++d) {
-                                o[d][n][x] *= alpha;
-                                o[d][n][x + 2] *= alpha;
-                            }
+                        for (int d = 0; d < DP / 16; ++d) {
+                            o[d][n][x] *= alpha;
+                            o[d][n][x + 2] *= alpha;
                         }
                     }
                 }
@@ -680,10 +690,10 @@ decode_tc_kernel(DecodeParams p, int groups) {
                         const float b = limit[n][x] == -INFINITY ? -INFINITY : base[n][x];
                         if (g == 0 && row < ng) {
                             if (!whole) { part.top(row) = b; part.sum(row) = sum; }
-                            else if (p.lse) p.lse[(int64_t)get.b * p.Hq + h * G + g0 + row] = b * kLn2 + logf(sum);
+                            else if (p.lse) p.lse[(int64_t)get.b * p.Hq + h * G + g0 + row] = lse_of(b, sum);
                         }
                         if (whole) {
-                            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                            const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
 #pragma unroll
                             for (int d = 0; d < DP / 16; ++d) {
                                 o[d][n][x] *= inv;
@@ -718,24 +728,14 @@ decode_tc_kernel(DecodeParams p, int groups) {
                 }
                 reset();
                 tile_in = 0;
-                if (!last) {
-                    if constexpr (kFetchQ) {
-#pragma unroll
-                        for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-                            for (int n = 0; n < NH; ++n) { q[k][n][0] = qn[k][n][0]; q[k][n][1] = qn[k][n][1]; }
-                    } else {
-                        load_q(nx, q);
-                    }
-                }
             }
-            get = nx;
+            get.next(p, groups);
         }
     }
     if (mine.early) {   // a head that ended while the ring was in use comes back
         __syncwarp();
         const float4* from = reinterpret_cast<const float4*>(ws.warp((int64_t)blockIdx.x * NW + warp).at);
-        for (int i = lane; i < MH * (p.D + 2) / 4; i += 32)
+        for (int i = lane; i < Part::floats(MH, p.D) / 4; i += 32)
             reinterpret_cast<float4*>(places + kPlace)[i] = from[i];
     }
     if (lane == 0) left[warp] = mine;
@@ -752,7 +752,7 @@ constexpr int kAnyTile = 16, kAnyWarps = 8, kAnyHeads = 4;
 
 __global__ void __launch_bounds__(kAnyWarps * 32)
 decode_any_kernel(DecodeParams p, int groups) {
-    constexpr int HG = kAnyHeads, kPlace = HG * (kMaxHeadDim + 2);
+    constexpr int HG = kAnyHeads, kPlace = Part::floats(HG, kMaxHeadDim);
     extern __shared__ __align__(128) char smem[];
     __shared__ Left left[kAnyWarps];
     sm100::grid_launch_dependents();
@@ -847,7 +847,7 @@ decode_any_kernel(DecodeParams p, int groups) {
             }
             if (lane == 0) {
                 if (!whole) { part.top(g) = m[g]; part.sum(g) = l[g]; }
-                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq] = m[g] * kLn2 + logf(l[g]);
+                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq] = lse_of(m[g], l[g]);
             }
         }
         tile0 = 0;
@@ -869,14 +869,16 @@ decode_any_kernel(DecodeParams p, int groups) {
 
 // ------------------------------------------------------------------------------------------
 // CTA (c, row): row `row` of the segment that goes on behind the run of decode CTA c, if one
-// does: its part there and one part of each CTA behind.  Each warp sums every kMergeWarps-th
-// part, and the warps' sums are added in order.
+// does: its part there and one part of each CTA behind, at most kCtas.  Every warp weighs all
+// parts (lane i: parts i, i + 32, ...) and sums those i = warp mod kMergeWarps; the warps'
+// sums are added in order.  All it does is wait for memory three times in a row (what is open,
+// the weights, the parts), so the loads of each step are issued together.
 // ------------------------------------------------------------------------------------------
-constexpr int kMergeWarps = 4;
+constexpr int kMergeWarps = 8, kMergeTurns = (kCtas + 31) / 32;
 
 __global__ void __launch_bounds__(kMergeWarps * 32)
 merge_kernel(DecodeParams p, int groups, int HG) {
-    __shared__ float s_top[kMergeWarps], s_sum[kMergeWarps], s_acc[kMergeWarps][kMaxHeadDim];
+    __shared__ float s_acc[kMergeWarps][kMaxHeadDim];
     sm100::grid_launch_dependents();
     sm100::grid_dependency_wait();
     const Workspace ws(p, HG);
@@ -884,62 +886,72 @@ merge_kernel(DecodeParams p, int groups, int HG) {
     const int4 open = ws.open[c];
     if (open.x < 0) return;
     const int G = p.Hq / p.Hkv;
-    const int b = open.x, h = open.y / groups, g0 = (open.y % groups) * HG, n = open.z + 1;
+    const int h = groups == 1 ? open.y : open.y / groups, g0 = (open.y - h * groups) * HG, n = open.z + 1;
     if (g0 + row >= G) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float2 ml[kMergeTurns];
     float top = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += kMergeWarps * 32) top = fmaxf(top, ws.cta(c + i, i == 0).top(row));
+#pragma unroll
+    for (int j = 0; j < kMergeTurns; ++j) {
+        const int i = j * 32 + lane;
+        ml[j] = i < n ? *reinterpret_cast<const float2*>(&ws.cta(c + i, i == 0).top(row)) : make_float2(-INFINITY, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < kMergeTurns; ++j) top = fmaxf(top, ml[j].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_top[w]);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[kMaxHeadDim / 32];
+    float sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < kMaxHeadDim / 32; ++x) acc[x] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < n; i += kMergeWarps) {
-        const Part part = ws.cta(c + i, i == 0);
-        const float a = sm100::ex2(part.top(row) - base);
-        sum += part.sum(row) * a;
-        const float* from = part.acc(row);
-#pragma unroll
-        for (int x = 0; x < kMaxHeadDim / 32; ++x)
-            if (lane + 32 * x < p.D) acc[x] += from[lane + 32 * x] * a;
+    for (int j = 0; j < kMergeTurns; ++j) {
+        ml[j].x = sm100::ex2(ml[j].x - base);
+        if (j * 32 + lane < n) sum += ml[j].x * ml[j].y;
     }
-    if (lane == 0) s_sum[warp] = sum;
 #pragma unroll
-    for (int x = 0; x < kMaxHeadDim / 32; ++x) s_acc[warp][lane + 32 * x] = acc[x];
-    __syncthreads();
-    float L = 0.f;
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) L += s_sum[w];
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int hq = h * G + g0 + row;
+    for (int d0 = 0; d0 < p.D; d0 += 64) {
+        const int d = d0 + lane * 2;
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < kMergeTurns; ++j) {
+            if (j * 32 >= n) break;
+#pragma unroll
+            for (int k = 0; k < 32 / kMergeWarps; ++k) {
+                const int i = j * 32 + k * kMergeWarps + warp;
+                const float a = __shfl_sync(0xffffffffu, ml[j].x, k * kMergeWarps + warp);
+                if (i < n && d < p.D) {
+                    const float* from = ws.cta(c + i, i == 0).acc(row) + d;
+                    acc.x = fmaf(from[0], a, acc.x);
+                    if (d + 1 < p.D) acc.y = fmaf(from[1], a, acc.y);
+                }
+            }
+        }
+        if (d < p.D) s_acc[warp][d] = acc.x;
+        if (d + 1 < p.D) s_acc[warp][d + 1] = acc.y;
+    }
+    __syncthreads();
     for (int d = threadIdx.x; d < p.D; d += kMergeWarps * 32) {
         float o = 0.f;
 #pragma unroll
         for (int w = 0; w < kMergeWarps; ++w) o += s_acc[w][d];
-        store_elt(p.out, (int64_t)b * p.o_stride_b + (int64_t)hq * p.o_stride_h + d, p.dtype,
-                  L == 0.f ? 0.f : o / L);
+        store_elt(p.out, (int64_t)open.x * p.o_stride_b + (int64_t)hq * p.o_stride_h + d, p.dtype,
+                  sum == 0.f ? 0.f : o / sum);
     }
-    if (p.lse && threadIdx.x == 0) p.lse[(int64_t)b * p.Hq + hq] = top * kLn2 + logf(L);
+    if (p.lse && threadIdx.x == 0) p.lse[(int64_t)open.x * p.Hq + hq] = lse_of(top, sum);
 }
 
 namespace {
 
-// 16-byte rows in the pool (its copies), 4-byte ones in q and out, token counts of 31 bits
+// 16-byte rows in the pool and in q (copies), 4-byte ones in out, token counts of 31 bits
 bool tc_ok(const DecodeParams& p) {
     if (p.dtype == RKV_F32 || p.D % 8) return false;
     if (p.W * p.P > 0x7fffff00 || p.P > 0x7fffffff) return false;
-    for (int64_t s : {p.stride_h, p.stride_p, p.stride_t})
+    for (int64_t s : {p.stride_h, p.stride_p, p.stride_t, p.q_stride_b, p.q_stride_h})
         if (s % 8) return false;
-    for (const void* ptr : {p.k, p.v})
+    for (const void* ptr : {p.k, p.v, p.q})
         if (reinterpret_cast<uintptr_t>(ptr) & 15) return false;
-    for (int64_t s : {p.q_stride_b, p.q_stride_h, p.o_stride_b, p.o_stride_h})
-        if (s % 2) return false;
-    return !((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out)) & 3);
+    return p.o_stride_b % 2 == 0 && p.o_stride_h % 2 == 0 && !(reinterpret_cast<uintptr_t>(p.out) & 3);
 }
 
 // A decode kernel and its merge, each launched so that its start overlaps the end of the kernel
@@ -971,9 +983,9 @@ cudaError_t launch_pair(Kernel kernel, int threads, int smem, const DecodeParams
 
 template <bool kBf16, int DP, int NH, bool kWhole>
 cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
-    constexpr int TT = DP <= 64 ? 32 : 16, NW = DP <= 128 ? 12 : 6, STAGES = 2;
-    using Shape = TcShape<DP, TT, NW, STAGES>;
-    static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 3072, "shared memory");
+    constexpr int TT = DP <= 64 ? 32 : 16, NW = DP <= 128 ? 12 - 2 * NH : 6 - NH, STAGES = 2;
+    using Shape = TcShape<DP, NH, TT, NW, STAGES>;
+    static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 4096, "shared memory");
     return launch_pair(decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>, NW * 32, Shape::kSmem, p,
                        NH * 8, st);
 }
@@ -999,7 +1011,7 @@ size_t decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D) {
 
 cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
     if (!tc_ok(p)) return launch_pair(decode_any_kernel, kAnyWarps * 32,
-                                       kAnyWarps * 2 * kAnyHeads * (kMaxHeadDim + 2) * (int)sizeof(float), p, kAnyHeads, st);
+                                       kAnyWarps * 2 * Part::floats(kAnyHeads, kMaxHeadDim) * 4, p, kAnyHeads, st);
     if (p.D <= 64) return launch_tc_heads<64>(p, st);
     if (p.D <= 128) return launch_tc_heads<128>(p, st);
     return launch_tc_heads<256>(p, st);

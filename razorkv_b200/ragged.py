@@ -267,7 +267,10 @@ def ragged_decode_attention(
     lse = torch.empty(B, H, dtype=torch.float32, device=dev) if return_lse else None
     if B == 0:
         return (out, lse) if return_lse else out
-    q = query if query.stride(3) == 1 else query.contiguous()
+    # rows of 16-byte steps, as the tensor-core kernels read them
+    q, step = query, 16 // query.element_size()
+    if q.stride(3) != 1 or q.stride(0) % step or q.stride(1) % step or q.data_ptr() & 15:
+        q = torch.empty(B, H, 1, D, dtype=q.dtype, device=dev).copy_(query)
     n = lengths.contiguous()
     first = starts.contiguous() if starts is not None else None
     if validate:
