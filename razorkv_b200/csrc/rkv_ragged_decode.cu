@@ -30,7 +30,7 @@ namespace ragged {
 static __device__ int g_error;
 
 constexpr int kCtas = 148;      // one persistent CTA per SM
-constexpr int kMostWarps = 12;  // warps per CTA of any kernel here (16 at most: join_parts)
+constexpr int kMostWarps = 8;   // warps per CTA of any kernel here (16 at most: join_parts)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -58,9 +58,10 @@ __device__ __forceinline__ int64_t tiles_of(int64_t first, int64_t last) {
 }
 
 // What a segment costs besides its tiles, in tiles: its queries, its outputs, the change of
-// pages.  Runs are of equal cost, so a segment of n tiles has n + kOver units, the first kOver of
-// which hold no tile.
-constexpr int kOver = 1;
+// pages.  Runs are of equal cost, so a segment of n tiles has n + over_of(TT) units, the first of
+// which hold no tile.  (64 requests of 1 to 4093 tokens: 38.7 us with 1, 38.2 with 2, 36.8 with 3
+// tiles of 16; 255 of up to 509: 26.3 us with 1, 28.4 with 2 tiles of 32.)
+__host__ __device__ constexpr int over_of(int tile_tokens) { return tile_tokens <= 16 ? 2 : 1; }
 
 // a / b of non-negative numbers, the 32-bit way where it can be
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
@@ -131,7 +132,7 @@ __device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_til
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
         range_of(p, b, &f, &l);
-        mine += (tiles_of<TT>(f, l) + kOver) * per_tile;
+        mine += (tiles_of<TT>(f, l) + over_of(TT)) * per_tile;
     }
     int64_t x = mine;
 #pragma unroll
@@ -141,6 +142,7 @@ __device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_til
     }
     if (lane == 31) s_sums[warp] = x;
     __syncthreads();
+    constexpr int kOver = over_of(TT);
     Runs r{};
     int64_t before = x - mine;
 #pragma unroll
@@ -745,6 +747,276 @@ decode_tc_kernel(DecodeParams p, int groups) {
 }
 
 // ------------------------------------------------------------------------------------------
+// fp32.  The same rings, with fp32 arithmetic (a product of tensor cores would round K and V to
+// fewer bits).  For the logits, LPT lanes share a token and read its row a quarter (half) each,
+// the queries come as broadcasts; for the output, a lane has DP / 32 dims of every head.  Both
+// halves are fused multiply-adds on pairs.  At HG heads per kv head that is 4 HG operations for
+// each 8 bytes read, a quarter of what the SMs could do while memory delivers them at HG = 8.
+// ------------------------------------------------------------------------------------------
+template <int DP, int HG, int TT, int NW, int STAGES>
+struct F32Shape {
+    static constexpr int kLpt = 32 / TT;                // lanes per token
+    static constexpr int kPitch = DP * 4 + 16 * kLpt;   // 8 lanes at a time read 128 different bytes
+    static constexpr int kPlane = TT * kPitch;
+    static constexpr int kStage = 2 * kPlane + HG * kPitch;
+    static constexpr int kSmem = NW * (STAGES * kStage + HG * kPitch);
+};
+
+template <int DP, int HG, int TT, int NW, int STAGES>
+__global__ void __launch_bounds__(NW * 32, 1)
+decode_f32_kernel(DecodeParams p, int groups) {
+    using Shape = F32Shape<DP, HG, TT, NW, STAGES>;
+    static_assert(HG % 4 == 0 && DP % 64 == 0 && (TT == 8 || TT == 16), "shape");
+    extern __shared__ __align__(128) char smem[];
+    __shared__ Left left[NW];
+    __shared__ __align__(16) float s_weight[NW][TT][HG];
+    constexpr int kLpt = Shape::kLpt;
+    constexpr int kChunks = DP / 4;                 // 16-byte chunks per row
+    constexpr int kCopies = TT * kChunks / 32;      // copies per lane for K, and for V
+    constexpr int kDims = DP / 32;                  // dims per lane of the output
+    constexpr int kPlace = STAGES * Shape::kStage / 8;
+    static_assert(kPlace >= Part::floats(HG, DP) && STAGES * Shape::kStage % 32 == 0, "two parts fit the ring");
+    sm100::grid_launch_dependents();
+    sm100::grid_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int G = p.Hq / p.Hkv;
+    const Workspace ws(p, HG);
+    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups);
+    if (blockIdx.x >= runs.ctas) {
+        if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        return;
+    }
+    const uint32_t ring = sm100::smem_u32(smem) + warp * STAGES * Shape::kStage;
+    float* places = reinterpret_cast<float*>(smem + warp * STAGES * Shape::kStage);
+    const float scale2 = p.scale * kLog2e, slack = kSlack / scale2;
+    Left mine{};
+    if (runs.count > 0) {
+        const int count = (int)runs.count;
+        Walk<TT> put, get;
+        put.start(runs, groups);
+        get = put;
+        int ahead = count;
+        const uint32_t P = (uint32_t)p.P;
+        int64_t window = 0;     // ids of 32 pages in a row, from page `win_at` of request win_b on
+        uint32_t win_at = 0;
+        int win_b = -1;
+        const char* kbytes = static_cast<const char*>(p.k);
+        const int64_t v_from_k = static_cast<const char*>(p.v) - kbytes;
+        bool with_q = true;     // queries come with the first tile of their segment
+        auto issue = [&](int stage) {
+            if (ahead > 0) {
+                const int t0 = put.token0();
+                const uint32_t dst = ring + stage * Shape::kStage;
+                if (with_q) {
+                    const int g0 = put.gi * HG, ng = min(HG, G - g0);
+                    const char* src = static_cast<const char*>(p.q) +
+                                      ((int64_t)put.b * p.q_stride_b + (int64_t)(put.h * G + g0) * p.q_stride_h) * 4;
+#pragma unroll
+                    for (int j = 0; j < HG * kChunks / 32; ++j) {
+                        const int i = lane + 32 * j, r = i / kChunks, c = i % kChunks;
+                        copy16_or_zero(dst + 2 * Shape::kPlane + r * Shape::kPitch + c * 16,
+                                       src + r * p.q_stride_h * 4 + c * 16, r < ng && c * 4 < p.D);
+                    }
+                }
+                const uint32_t p0 = p.div_p(max(t0, put.first));
+                const uint32_t p1 = p.div_p(max(min(t0 + TT, put.last) - 1, 0));
+                if (put.last > put.first && (put.b != win_b || p0 < win_at || p1 >= win_at + 32)) {
+                    win_b = put.b;
+                    win_at = p0;
+                    const int64_t at = (int64_t)p0 + lane;
+                    window = at * P < put.last ? p.table[(int64_t)put.b * p.table_stride + at] : 0;
+                    if (window < 0 || window >= p.num_slots) { atomicMax(&g_error, kErrPage); window = 0; }
+                }
+                // byte offset of row `lane` of the tile in the pool
+                const int tr = t0 + lane;
+                const uint32_t pr = p.div_p(tr);
+                const int64_t page = __shfl_sync(0xffffffffu, window, pr - win_at);
+                const int64_t row = (page * p.stride_p + (int64_t)((uint32_t)tr - pr * P) * p.stride_t +
+                                     (int64_t)put.h * p.stride_h) * 4;
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j) {
+                    const int i = lane + 32 * j, r = i / kChunks, c = i % kChunks;
+                    const bool on = t0 + r >= put.first && t0 + r < put.last && c * 4 < p.D;
+                    const char* src = kbytes + __shfl_sync(0xffffffffu, row, r) + c * 16;
+                    copy16_or_zero(dst + r * Shape::kPitch + c * 16, src, on);
+                    copy16_or_zero(dst + Shape::kPlane + r * Shape::kPitch + c * 16, src + v_from_k, on);
+                }
+                --ahead;
+                put.next(p, groups);
+                with_q = put.tile == 0;
+            }
+            copies_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) issue(s);
+
+        const int tok = lane / kLpt, share = lane % kLpt;
+        uint64_t o[HG][kDims / 2];
+        float base[HG], limit[HG], l[HG];
+        auto reset = [&]() {
+#pragma unroll
+            for (int g = 0; g < HG; ++g) {
+                base[g] = 0.f; limit[g] = -INFINITY; l[g] = 0.f;
+#pragma unroll
+                for (int x = 0; x < kDims / 2; ++x) o[g][x] = 0;
+            }
+        };
+        reset();
+        const uint32_t k_lane = ring + tok * Shape::kPitch + share * 16;
+        // dims of this lane: two, or fours that are 128 apart
+        const uint32_t v_lane = ring + Shape::kPlane + lane * (kDims == 2 ? 8 : 16);
+        int tile_in = get.tile, stage = 0;
+        // the queries are moved from the stage that brought them to a place behind the rings
+        float* q_own = reinterpret_cast<float*>(smem + NW * STAGES * Shape::kStage) + warp * HG * (Shape::kPitch / 4);
+        const uint32_t q_base = sm100::smem_u32(q_own) + share * 16;
+        for (int i = 0; i < count; ++i) {
+            copies_wait<STAGES - 1>();
+            __syncwarp();
+            const uint32_t at = stage * Shape::kStage;
+            if (get.tile == tile_in) {
+                for (int x = lane; x < HG * Shape::kPitch / 16; x += 32)
+                    reinterpret_cast<uint4*>(q_own)[x] = sm100::lds128(ring + at + 2 * Shape::kPlane + x * 16);
+                __syncwarp();
+            }
+            uint64_t s2[HG];
+#pragma unroll
+            for (int g = 0; g < HG; ++g) s2[g] = 0;
+#pragma unroll
+            for (int j = 0; j < kChunks / kLpt; ++j) {
+                const uint4 k = sm100::lds128(k_lane + at + j * kLpt * 16);
+                const uint64_t k0 = (uint64_t)k.y << 32 | k.x, k1 = (uint64_t)k.w << 32 | k.z;
+#pragma unroll
+                for (int g = 0; g < HG; ++g) {
+                    const uint4 q = sm100::lds128(q_base + g * Shape::kPitch + j * kLpt * 16);
+                    sm100::ffma2(s2[g], (uint64_t)q.y << 32 | q.x, k0);
+                    sm100::ffma2(s2[g], (uint64_t)q.w << 32 | q.z, k1);
+                }
+            }
+            const int t = get.token0() + tok;
+            const bool in = t >= get.first && t < get.last;
+            float s[HG];
+            bool over = false;
+#pragma unroll
+            for (int g = 0; g < HG; ++g) {
+                float v = sm100::sum_pair(s2[g]);
+#pragma unroll
+                for (int x = kLpt / 2; x > 0; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+                s[g] = in ? v : -INFINITY;
+                over = over || s[g] > limit[g];
+            }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int g = 0; g < HG; ++g) {
+                    float v = s[g];
+#pragma unroll
+                    for (int x = 16; x >= kLpt; x >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+                    const bool renew = v > limit[g];
+                    const float b = v * scale2;
+                    const float alpha = !renew ? 1.f : limit[g] == -INFINITY ? 0.f : sm100::ex2(base[g] - b);
+                    base[g] = renew ? b : base[g];
+                    limit[g] = renew ? v + slack : limit[g];
+                    l[g] *= alpha;
+#pragma unroll
+                    for (int x = 0; x < kDims / 2; ++x) o[g][x] = sm100::fmul2(o[g][x], sm100::pack2(alpha, alpha));
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < HG; ++g) {
+                s[g] = sm100::ex2(fmaf(s[g], scale2, -base[g]));
+                l[g] += s[g];
+            }
+            if (share == 0) {
+#pragma unroll
+                for (int g = 0; g < HG; g += 4)
+                    *reinterpret_cast<float4*>(&s_weight[warp][tok][g]) = make_float4(s[g], s[g + 1], s[g + 2], s[g + 3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int y = 0; y < TT; ++y) {
+                uint64_t v[kDims / 2];
+                if constexpr (kDims == 2) {
+                    v[0] = (uint64_t)sm100::lds32(v_lane + at + y * Shape::kPitch + 4) << 32 |
+                           sm100::lds32(v_lane + at + y * Shape::kPitch);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < kDims / 4; ++x) {
+                        const uint4 f = sm100::lds128(v_lane + at + y * Shape::kPitch + x * 512);
+                        v[2 * x] = (uint64_t)f.y << 32 | f.x;
+                        v[2 * x + 1] = (uint64_t)f.w << 32 | f.z;
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < HG; g += 4) {
+                    const float4 w = *reinterpret_cast<const float4*>(&s_weight[warp][y][g]);
+#pragma unroll
+                    for (int x = 0; x < kDims / 2; ++x) {
+                        sm100::ffma2(o[g][x], sm100::pack2(w.x, w.x), v[x]);
+                        sm100::ffma2(o[g + 1][x], sm100::pack2(w.y, w.y), v[x]);
+                        sm100::ffma2(o[g + 2][x], sm100::pack2(w.z, w.z), v[x]);
+                        sm100::ffma2(o[g + 3][x], sm100::pack2(w.w, w.w), v[x]);
+                    }
+                }
+            }
+            __syncwarp();
+            issue(stage);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+            // ---- the end of the segment, or of the run
+            const bool ends = get.tile + 1 == get.tiles, last = i + 1 == count;
+            if (ends || last) {
+                const bool whole = tile_in == 0 && ends;
+                const int h = get.h, g0 = get.gi * HG;
+                const int ng = min(HG, G - g0);
+                if (!whole) {
+                    if (tile_in > 0) {
+                        mine.head = 1; mine.ends = ends; mine.early = !last;
+                        mine.head_b = get.b; mine.head_seg = h * groups + get.gi;
+                    } else {
+                        mine.tail = 1; mine.tail_b = get.b; mine.tail_seg = h * groups + get.gi;
+                    }
+                    mine.rest = get.tiles - get.tile - 1;
+                }
+                const Part part = last ? Part{places, HG, p.D} : ws.warp((int64_t)blockIdx.x * NW + warp);
+#pragma unroll
+                for (int g = 0; g < HG; ++g) {
+                    float sum = l[g];
+#pragma unroll
+                    for (int x = 16; x >= kLpt; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                    if (g >= ng) break;
+                    const int hq = h * G + g0 + g;
+                    const float b = limit[g] == -INFINITY ? -INFINITY : base[g];
+                    if (lane == 0) {
+                        if (!whole) { part.top(g) = b; part.sum(g) = sum; }
+                        else if (p.lse) p.lse[(int64_t)get.b * p.Hq + hq] = lse_of(b, sum);
+                    }
+                    const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+                    float* to = whole ? static_cast<float*>(p.out) + (int64_t)get.b * p.o_stride_b + (int64_t)hq * p.o_stride_h
+                                      : part.acc(g);
+#pragma unroll
+                    for (int x = 0; x < kDims / 2; ++x) {
+                        const int d = kDims == 2 ? lane * 2 : (x / 2) * 128 + lane * 4 + (x % 2) * 2;
+                        const uint64_t v = sm100::fmul2(o[g][x], sm100::pack2(inv, inv));
+                        if (d < p.D) *reinterpret_cast<uint64_t*>(to + d) = v;
+                    }
+                }
+                reset();
+                tile_in = 0;
+            }
+            get.next(p, groups);
+        }
+    }
+    if (mine.early) {   // a head that ended while the ring was in use comes back
+        __syncwarp();
+        const float4* from = reinterpret_cast<const float4*>(ws.warp((int64_t)blockIdx.x * NW + warp).at);
+        for (int i = lane; i < Part::floats(HG, p.D) / 4; i += 32)
+            reinterpret_cast<float4*>(places + kPlace)[i] = from[i];
+    }
+    if (lane == 0) left[warp] = mine;
+    __syncthreads();
+    join_parts<NW, HG, RKV_F32>(p, runs, ws, left, reinterpret_cast<float*>(smem), 2 * kPlace, kPlace, groups);
+}
+
+// ------------------------------------------------------------------------------------------
 // Every other shape: any alignment, head_dim up to 256.  Lanes share the elements of a row; a
 // token's logit is a sum over the warp.
 // ------------------------------------------------------------------------------------------
@@ -869,76 +1141,89 @@ decode_any_kernel(DecodeParams p, int groups) {
 
 // ------------------------------------------------------------------------------------------
 // CTA (c, row): row `row` of the segment that goes on behind the run of decode CTA c, if one
-// does: its part there and one part of each CTA behind, at most kCtas.  Every warp weighs all
-// parts (lane i: parts i, i + 32, ...) and sums those i = warp mod kMergeWarps; the warps'
-// sums are added in order.  All it does is wait for memory three times in a row (what is open,
-// the weights, the parts), so the loads of each step are issued together.
+// does: its part there and one part of each CTA behind, at most kCtas in all.  A thread per part
+// weighs it, and warp w sums the parts w, w + kMergeWarps, ..., whose sums are added in order.
+// All of it is waiting for memory, so the first kMergeAhead parts of each warp are on their way
+// before the weights are known.
 // ------------------------------------------------------------------------------------------
-constexpr int kMergeWarps = 8, kMergeTurns = (kCtas + 31) / 32;
+constexpr int kMergeWarps = 8, kMergeAhead = 5;
+static_assert(kMergeWarps * 32 >= kCtas && kMergeWarps * 32 >= kMaxHeadDim, "a thread per part");
 
 __global__ void __launch_bounds__(kMergeWarps * 32)
 merge_kernel(DecodeParams p, int groups, int HG) {
+    __shared__ float s_weight[kMergeWarps * 32], s_top[kMergeWarps], s_sum[kMergeWarps];
     __shared__ float s_acc[kMergeWarps][kMaxHeadDim];
     sm100::grid_launch_dependents();
     sm100::grid_dependency_wait();
     const Workspace ws(p, HG);
-    const int c = blockIdx.x, row = blockIdx.y;
+    const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     const int4 open = ws.open[c];
     if (open.x < 0) return;
     const int G = p.Hq / p.Hkv;
     const int h = groups == 1 ? open.y : open.y / groups, g0 = (open.y - h * groups) * HG, n = open.z + 1;
     if (g0 + row >= G) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float2 ml[kMergeTurns];
-    float top = -INFINITY;
+    const int lane = tid & 31, warp = tid >> 5;
+    // part 0 is the open one of CTA c, part i > 0 the first of CTA c + i
+    const float* parts = ws.cta(c, 0).at;
+    auto at = [&](int i) { return parts + (2 * i + (i == 0)) * ws.stride; };
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (tid < n) ml = *reinterpret_cast<const float2*>(&Part{const_cast<float*>(at(tid)), HG, p.D}.top(row));
+    const int skip = 2 * HG + row * (p.D + 4) + lane;
+    float ahead[kMergeAhead][4];
 #pragma unroll
-    for (int j = 0; j < kMergeTurns; ++j) {
-        const int i = j * 32 + lane;
-        ml[j] = i < n ? *reinterpret_cast<const float2*>(&ws.cta(c + i, i == 0).top(row)) : make_float2(-INFINITY, 0.f);
+    for (int k = 0; k < kMergeAhead; ++k) {
+        const float* f = at(min(warp + k * kMergeWarps, n - 1)) + skip;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) ahead[k][x] = lane + 32 * x < p.D ? f[32 * x] : 0.f;
     }
-#pragma unroll
-    for (int j = 0; j < kMergeTurns; ++j) top = fmaxf(top, ml[j].x);
+    float top = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kMergeTurns; ++j) {
-        ml[j].x = sm100::ex2(ml[j].x - base);
-        if (j * 32 + lane < n) sum += ml[j].x * ml[j].y;
-    }
+    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_top[w]);
+    const float weight = sm100::ex2(ml.x - (top == -INFINITY ? 0.f : top));
+    s_weight[tid] = weight;
+    float sum = tid < n ? ml.y * weight : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const int hq = h * G + g0 + row;
-    for (int d0 = 0; d0 < p.D; d0 += 64) {
-        const int d = d0 + lane * 2;
-        float2 acc = make_float2(0.f, 0.f);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < kMergeTurns; ++j) {
-            if (j * 32 >= n) break;
+    for (int w = 0; w < kMergeWarps; ++w) sum += s_sum[w];
+    for (int x0 = 0; x0 * 32 < p.D; x0 += 4) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        int i = warp;
+        if (x0 == 0) {
 #pragma unroll
-            for (int k = 0; k < 32 / kMergeWarps; ++k) {
-                const int i = j * 32 + k * kMergeWarps + warp;
-                const float a = __shfl_sync(0xffffffffu, ml[j].x, k * kMergeWarps + warp);
-                if (i < n && d < p.D) {
-                    const float* from = ws.cta(c + i, i == 0).acc(row) + d;
-                    acc.x = fmaf(from[0], a, acc.x);
-                    if (d + 1 < p.D) acc.y = fmaf(from[1], a, acc.y);
-                }
-            }
+            for (int k = 0; k < kMergeAhead; ++k, i += kMergeWarps)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (i < n) acc[x] = fmaf(ahead[k][x], s_weight[i], acc[x]);
         }
-        if (d < p.D) s_acc[warp][d] = acc.x;
-        if (d + 1 < p.D) s_acc[warp][d + 1] = acc.y;
+#pragma unroll 4
+        for (; i < n; i += kMergeWarps) {
+            const float* f = at(i) + skip + 32 * x0;
+            const float a = s_weight[i];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (lane + 32 * (x0 + x) < p.D) acc[x] = fmaf(f[32 * x], a, acc[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s_acc[warp][lane + 32 * (x0 + x)] = acc[x];
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < p.D; d += kMergeWarps * 32) {
+    const int hq = h * G + g0 + row;
+    if (tid < p.D) {
         float o = 0.f;
 #pragma unroll
-        for (int w = 0; w < kMergeWarps; ++w) o += s_acc[w][d];
-        store_elt(p.out, (int64_t)open.x * p.o_stride_b + (int64_t)hq * p.o_stride_h + d, p.dtype,
+        for (int w = 0; w < kMergeWarps; ++w) o += s_acc[w][tid];
+        store_elt(p.out, (int64_t)open.x * p.o_stride_b + (int64_t)hq * p.o_stride_h + tid, p.dtype,
                   sum == 0.f ? 0.f : o / sum);
     }
-    if (p.lse && threadIdx.x == 0) p.lse[(int64_t)open.x * p.Hq + hq] = lse_of(top, sum);
+    if (p.lse && tid == 0) p.lse[(int64_t)open.x * p.Hq + hq] = lse_of(top, sum);
 }
 
 namespace {
@@ -983,7 +1268,7 @@ cudaError_t launch_pair(Kernel kernel, int threads, int smem, const DecodeParams
 
 template <bool kBf16, int DP, int NH, bool kWhole>
 cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
-    constexpr int TT = DP <= 64 ? 32 : 16, NW = DP <= 128 ? 12 - 2 * NH : 6 - NH, STAGES = 2;
+    constexpr int TT = DP <= 64 ? 32 : 16, NW = DP <= 128 ? 8 : 6 - NH, STAGES = 2;
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 4096, "shared memory");
     return launch_pair(decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>, NW * 32, Shape::kSmem, p,
@@ -1002,6 +1287,30 @@ cudaError_t launch_tc_heads(const DecodeParams& p, cudaStream_t st) {
     return p.Hq / p.Hkv > 8 ? launch_tc_dim<DP, 2>(p, st) : launch_tc_dim<DP, 1>(p, st);
 }
 
+// The same for fp32, with rows of 16 bytes in out
+bool f32_ok(const DecodeParams& p) {
+    if (p.dtype != RKV_F32 || p.D % 4) return false;
+    if (p.W * p.P > 0x7fffff00 || p.P > 0x7fffffff) return false;
+    for (int64_t s : {p.stride_h, p.stride_p, p.stride_t, p.q_stride_b, p.q_stride_h, p.o_stride_b, p.o_stride_h})
+        if (s % 4) return false;
+    for (const void* ptr : {p.k, p.v, p.q, (const void*)p.out})
+        if (reinterpret_cast<uintptr_t>(ptr) & 15) return false;
+    return true;
+}
+
+template <int DP, int HG>
+cudaError_t launch_f32(const DecodeParams& p, cudaStream_t st) {
+    constexpr int TT = DP <= 64 ? 16 : 8, NW = DP <= 128 ? 10 - HG / 2 : 5 - HG / 4, STAGES = 2;
+    using Shape = F32Shape<DP, HG, TT, NW, STAGES>;
+    static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 8192, "shared memory");
+    return launch_pair(decode_f32_kernel<DP, HG, TT, NW, STAGES>, NW * 32, Shape::kSmem, p, HG, st);
+}
+
+template <int DP>
+cudaError_t launch_f32_heads(const DecodeParams& p, cudaStream_t st) {
+    return p.Hq / p.Hkv > 4 ? launch_f32<DP, 8>(p, st) : launch_f32<DP, 4>(p, st);
+}
+
 }  // namespace
 
 // Upper bound over the kernels that a call of these sizes may take.
@@ -1010,6 +1319,11 @@ size_t decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D) {
 }
 
 cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
+    if (f32_ok(p)) {
+        if (p.D <= 64) return launch_f32_heads<64>(p, st);
+        if (p.D <= 128) return launch_f32_heads<128>(p, st);
+        return launch_f32_heads<256>(p, st);
+    }
     if (!tc_ok(p)) return launch_pair(decode_any_kernel, kAnyWarps * 32,
                                        kAnyWarps * 2 * Part::floats(kAnyHeads, kMaxHeadDim) * 4, p, kAnyHeads, st);
     if (p.D <= 64) return launch_tc_heads<64>(p, st);
