@@ -46,7 +46,10 @@ int rkv_ragged_page_tables(const int64_t* lengths, const int64_t* new_lengths, i
     if (max_new_tokens > 0 && (!slot_map || !positions)) return RKV_ERR_INVALID_ARGUMENT;
     ragged::TableParams p{lengths, new_lengths, requests, page_size, page_table, pt_stride, pt_width,
                           ring, ring_size, state, out_lengths, out_state, slot_map, positions,
-                          max_new_tokens, token_starts};
+                          max_new_tokens, token_starts, 0, 0, ragged::FastDiv()};
+    p.in_place = out_lengths == lengths || out_lengths == new_lengths || out_state == state;
+    p.narrow = pt_width * page_size < (1ll << 31);
+    if (p.narrow) p.div_p = ragged::FastDiv((uint32_t)(page_size < (1ll << 31) ? page_size : 1));
     return status_of(ragged::launch_tables(p, S(stream)));
 }
 
@@ -61,7 +64,9 @@ int rkv_ragged_append(const rkv_kv_layout* pool, const void* k_new, const void* 
     ragged::AppendParams p{const_cast<void*>(pool->k), const_cast<void*>(pool->v), pool->stride_h,
                            pool->stride_p, pool->stride_t, pool->page_size, pool->num_slots,
                            k_new, v_new, new_stride_t, new_stride_h, n_new, slot_map,
-                           (int)pool->num_kv_heads, pool->head_dim, pool->dtype};
+                           (int)pool->num_kv_heads, pool->head_dim, pool->dtype,
+                           pool->page_size < (1ll << 31), ragged::FastDiv()};
+    if (p.narrow) p.div_p = ragged::FastDiv((uint32_t)pool->page_size);
     return status_of(ragged::launch_append(p, S(stream)));
 }
 

@@ -36,12 +36,15 @@ struct TableParams {
     int64_t* ring; int64_t C; int64_t* state;
     int64_t* out_lengths; int64_t* out_state;
     int64_t* slot_map; int64_t* positions; int64_t M; int64_t* starts;
+    int in_place;               // an output is an input: written when every CTA has read it
+    int narrow; FastDiv div_p;  // W * P below 2^31: division by P
 };
 
 struct AppendParams {
     void* k; void* v; int64_t stride_h, stride_p, stride_t, P, num_slots;
     const void* k_new; const void* v_new; int64_t new_stride_t, new_stride_h;
     int64_t T; const int64_t* slot_map; int Hkv, D, dtype;
+    int narrow; FastDiv div_p;  // P below 2^31: division of such a slot by P
 };
 
 struct DecodeParams {

@@ -19,6 +19,8 @@
 // workspace has to be set before the call.
 #include <math.h>
 
+#include <atomic>
+
 #include "rkv_common.cuh"
 #include "rkv_kernels.h"
 #include "rkv_ragged.h"
@@ -1241,12 +1243,18 @@ bool tc_ok(const DecodeParams& p) {
 
 // A decode kernel and its merge, each launched so that its start overlaps the end of the kernel
 // before it (both wait for that kernel's results first).
-template <typename Kernel>
-cudaError_t launch_pair(Kernel kernel, int threads, int smem, const DecodeParams& p, int HG, cudaStream_t st) {
+template <void (*kernel)(DecodeParams, int)>
+cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, cudaStream_t st) {
     const int groups = (p.Hq / p.Hkv + HG - 1) / HG;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the kernel's shared memory is set once per device (a setting of the function, not of a call)
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(set.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
+        if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_release);
     }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1258,7 +1266,7 @@ cudaError_t launch_pair(Kernel kernel, int threads, int smem, const DecodeParams
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = counted(cudaLaunchKernelEx(&cfg, kernel, p, groups), 1);
+    e = counted(cudaLaunchKernelEx(&cfg, kernel, p, groups), 1);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(kCtas, HG);
     cfg.blockDim = dim3(kMergeWarps * 32);
@@ -1271,8 +1279,7 @@ cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
     constexpr int TT = DP <= 64 ? 32 : 16, NW = DP <= 128 ? 8 : 6 - NH, STAGES = 2;
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 4096, "shared memory");
-    return launch_pair(decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>, NW * 32, Shape::kSmem, p,
-                       NH * 8, st);
+    return launch_pair<decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>>(NW * 32, Shape::kSmem, p, NH * 8, st);
 }
 
 template <int DP, int NH>
@@ -1303,7 +1310,7 @@ cudaError_t launch_f32(const DecodeParams& p, cudaStream_t st) {
     constexpr int TT = DP <= 64 ? 16 : 8, NW = DP <= 128 ? 10 - HG / 2 : 5 - HG / 4, STAGES = 2;
     using Shape = F32Shape<DP, HG, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 8192, "shared memory");
-    return launch_pair(decode_f32_kernel<DP, HG, TT, NW, STAGES>, NW * 32, Shape::kSmem, p, HG, st);
+    return launch_pair<decode_f32_kernel<DP, HG, TT, NW, STAGES>>(NW * 32, Shape::kSmem, p, HG, st);
 }
 
 template <int DP>
@@ -1324,7 +1331,7 @@ cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
         if (p.D <= 128) return launch_f32_heads<128>(p, st);
         return launch_f32_heads<256>(p, st);
     }
-    if (!tc_ok(p)) return launch_pair(decode_any_kernel, kAnyWarps * 32,
+    if (!tc_ok(p)) return launch_pair<decode_any_kernel>(kAnyWarps * 32,
                                        kAnyWarps * 2 * Part::floats(kAnyHeads, kMaxHeadDim) * 4, p, kAnyHeads, st);
     if (p.D <= 64) return launch_tc_heads<64>(p, st);
     if (p.D <= 128) return launch_tc_heads<128>(p, st);

@@ -5,6 +5,7 @@
 #include "rkv_common.cuh"
 #include "rkv_kernels.h"
 #include "rkv_ragged.h"
+#include "rkv_sm100.cuh"
 
 namespace rkv {
 namespace ragged {
@@ -26,8 +27,9 @@ static __device__ int g_error;
 // per entry) and of kChunk returned pages.  A chunk finds the request of each entry from
 // marks: the thread that owns a request marks the entry where it starts, and a running
 // maximum over the chunk carries the mark to the entries behind it.
-// The state may be updated in place: it is written by the last CTA to finish, after every CTA
-// has read it (a ticket in the state's third word, which returns to zero).
+// The lengths and the state may be updated in place: then they are written by the last CTA to
+// finish, after every CTA has read them (a ticket in the state's third word, which returns to
+// zero); otherwise by the first CTA, without waiting.
 // ------------------------------------------------------------------------------------------
 constexpr int kThreads = 1024;
 constexpr int kChunk = kThreads;
@@ -35,6 +37,19 @@ constexpr int kChunk = kThreads;
 struct Sums {
     int64_t need, give, fresh;
 };
+
+// x / P for 0 <= x <= capacity, which is below 2^31 where the divisor is set
+struct Pages {
+    FastDiv div; int64_t P; bool narrow;
+    __device__ __forceinline__ int64_t of(int64_t x) const { return narrow ? (int64_t)div((uint32_t)x) : x / P; }
+    __device__ __forceinline__ int64_t up(int64_t x) const { return of(x) + (of(x) * P < x); }
+};
+
+// x mod C for 0 <= x < 3 C
+__device__ __forceinline__ int64_t wrap(int64_t x, int64_t C) {
+    x -= x >= C ? C : 0;
+    return x - (x >= C ? C : 0);
+}
 
 __device__ __forceinline__ int64_t shfl_up64(int64_t v, int o) {
     return __shfl_up_sync(0xffffffffu, v, o);
@@ -91,9 +106,12 @@ tables_kernel(TableParams p) {
     __shared__ int mark[kChunk];           // entry at which a request starts, or -1
     __shared__ int64_t mark_req[kChunk], mark_at[kChunk], mark_pages[kChunk];
     __shared__ int s_last;
+    sm100::grid_launch_dependents();
+    sm100::grid_dependency_wait();
     const int tid = threadIdx.x;
     const int64_t head = p.state[0], count = p.state[1];
     const int64_t capacity = p.W * p.P;
+    const Pages pages{p.div_p, p.P, p.narrow != 0};
     const int64_t per = (p.R + kThreads - 1) / kThreads;
     const int64_t r0 = min(p.R, tid * per), r1 = min(p.R, r0 + per);
 
@@ -102,7 +120,7 @@ tables_kernel(TableParams p) {
     for (int64_t r = r0; r < r1; ++r) {
         const int64_t n = p.lengths[r], m = p.new_lengths[r];
         if (n < 0 || n > capacity || m < 0 || m > capacity) { bad = 1; continue; }
-        const int64_t have = (n + p.P - 1) / p.P, want = (m + p.P - 1) / p.P;
+        const int64_t have = pages.up(n), want = pages.up(m);
         mine.need += max((int64_t)0, want - have);
         mine.give += max((int64_t)0, have - want);
         mine.fresh += max((int64_t)0, m - n);
@@ -135,7 +153,7 @@ tables_kernel(TableParams p) {
                     mark_req[at] = r; mark_at[at] = s; mark_pages[at] = a;
                 }
                 s += m - n;
-                a += max((int64_t)0, (m + p.P - 1) / p.P - (n + p.P - 1) / p.P);
+                a += pages.up(m) - pages.up(n);
             }
         }
         __syncthreads();
@@ -144,9 +162,9 @@ tables_kernel(TableParams p) {
         if (i >= total.fresh) { p.slot_map[i] = -1; p.positions[i] = 0; continue; }
         const int64_t r = mark_req[at];
         const int64_t n = p.lengths[r], t = n + (i - mark_at[at]);
-        const int64_t j = t / p.P, off = t - j * p.P, have = (n + p.P - 1) / p.P;
+        const int64_t j = pages.of(t), off = t - j * p.P, have = pages.up(n);
         int64_t* entry = p.table + r * p.table_stride + j;
-        const int64_t page = j < have ? *entry : p.ring[(head + mark_pages[at] + j - have) % p.C];
+        const int64_t page = j < have ? *entry : p.ring[wrap(head + mark_pages[at] + j - have, p.C)];
         const bool inside = page >= 0 && page < p.C;
         if (!inside) atomicMax(&g_error, kErrPage);
         if (j >= have && off == 0) *entry = page;
@@ -164,8 +182,7 @@ tables_kernel(TableParams p) {
             if (base.give < c0 + kChunk && base.give + mine.give > c0) {
                 int64_t g = base.give;
                 for (int64_t r = r0; r < r1 && g < c0 + kChunk; ++r) {
-                    const int64_t have = (p.lengths[r] + p.P - 1) / p.P;
-                    const int64_t want = (p.new_lengths[r] + p.P - 1) / p.P;
+                    const int64_t have = pages.up(p.lengths[r]), want = pages.up(p.new_lengths[r]);
                     if (want >= have) continue;
                     if (g + (have - want) > c0) {
                         const int at = (int)max((int64_t)0, g - c0);
@@ -179,13 +196,15 @@ tables_kernel(TableParams p) {
             const int at = block_running_max(mark[tid], warp_max);
             const int64_t i = c0 + tid;
             if (i >= total.give) continue;
-            p.ring[(head + count + i) % p.C] =
+            p.ring[wrap(head + count + i, p.C)] =
                 p.table[mark_req[at] * p.table_stride + mark_pages[at] + (i - mark_at[at])];
         }
     }
 
-    // token starts, lengths and state: the last CTA, so that they may replace the inputs
-    if (gridDim.x > 1) {
+    // token starts, lengths and state
+    if (!p.in_place) {
+        if (blockIdx.x > 0) return;
+    } else if (gridDim.x > 1) {
         __syncthreads();
         if (tid == 0) {
             __threadfence();
@@ -205,47 +224,89 @@ tables_kernel(TableParams p) {
     }
     if (tid == 0) {
         p.starts[p.R] = ok ? total.fresh : 0;
-        p.out_state[0] = ok ? (head + total.need) % p.C : head;
+        p.out_state[0] = ok ? wrap(head + total.need, p.C) : head;
         p.out_state[1] = ok ? count - total.need + total.give : count;
         p.out_state[2] = 0;
         if (!ok) atomicMax(&g_error, kErrRefused);
     }
 }
 
+namespace {
+
+// Launches so that the start overlaps the end of the kernel before, for whose results the kernel
+// waits first.
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), int64_t ctas, int threads, cudaStream_t st, const A&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return counted(cudaLaunchKernelEx(&cfg, kernel, args...), 1);
+}
+
+}  // namespace
+
 cudaError_t launch_tables(const TableParams& p, cudaStream_t st) {
-    int64_t ctas = (p.M + kChunk - 1) / kChunk;
-    if (ctas < 1) ctas = 1;
-    if (ctas > 148) ctas = 148;
-    tables_kernel<<<(unsigned)ctas, kThreads, 0, st>>>(p);
-    return counted(cudaGetLastError(), 1);
+    // a CTA per chunk of new tokens, or per 16 chunks of pages that may come back
+    const double back = (double)p.R * (double)p.W / (16 * kChunk), fresh = ((double)p.M + kChunk - 1) / kChunk;
+    const double ctas = back > fresh ? back : fresh;
+    return launch(tables_kernel, ctas < 1 ? 1 : ctas > 148 ? 148 : (int64_t)ctas, kThreads, st, p);
 }
 
 // ------------------------------------------------------------------------------------------
-// Append: row (t, h) of k_new / v_new to slot slot_map[t] of the pool.
+// Append: row (t, h) of k_new / v_new to slot slot_map[t] of the pool, in pieces of a Vec.  A
+// thread has kPieces pieces of K and of V on their way at a time.
 // ------------------------------------------------------------------------------------------
+constexpr int kAppendThreads = 256, kPieces = 4;
+
 template <typename Vec>
-__global__ void __launch_bounds__(256)
-append_kernel(AppendParams p, int chunks, int elts, int64_t tokens_per_cta) {
+__global__ void __launch_bounds__(kAppendThreads)
+append_kernel(AppendParams p, FastDiv div_token, FastDiv div_row, int per_token, int per_row, int elts,
+              int tokens_per_cta) {
+    sm100::grid_launch_dependents();
+    sm100::grid_dependency_wait();
     const Vec* kn = static_cast<const Vec*>(p.k_new);
     const Vec* vn = static_cast<const Vec*>(p.v_new);
     Vec* k = static_cast<Vec*>(p.k);
     Vec* v = static_cast<Vec*>(p.v);
-    const int64_t t0 = blockIdx.x * tokens_per_cta;
-    const int per_token = p.Hkv * chunks;
-    const int n = (int)min(tokens_per_cta, p.T - t0) * per_token;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const int tl = i / per_token, rest = i - tl * per_token;
-        const int h = rest / chunks, c = rest - h * chunks;
-        const int64_t t = t0 + tl;
-        const int64_t slot = p.slot_map[t];
-        if (slot < 0) continue;
-        const int64_t page = slot / p.P;
-        if (page >= p.num_slots) { atomicMax(&g_error, kErrPage); continue; }
-        const int64_t src = (t * p.new_stride_t + h * p.new_stride_h) / elts + c;
-        const int64_t dst = (page * p.stride_p + (slot - page * p.P) * p.stride_t +
-                             h * p.stride_h) / elts + c;
-        k[dst] = kn[src];
-        v[dst] = vn[src];
+    const int64_t t0 = (int64_t)blockIdx.x * tokens_per_cta;
+    const int n = (int)min((int64_t)tokens_per_cta, p.T - t0) * per_token;
+    for (int i0 = threadIdx.x; i0 < n; i0 += kAppendThreads * kPieces) {
+        int64_t slot[kPieces], src[kPieces];
+        int in_row[kPieces], head[kPieces];
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+            const int i = i0 + u * kAppendThreads;
+            const int tl = div_token(i), rest = i - tl * per_token;
+            head[u] = div_row(rest);
+            in_row[u] = rest - head[u] * per_row;
+            const int64_t t = t0 + tl;
+            slot[u] = i < n ? p.slot_map[t] : -1;
+            src[u] = (t * p.new_stride_t + head[u] * p.new_stride_h) / elts + in_row[u];
+        }
+        Vec a[kPieces], b[kPieces];
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+            if (slot[u] < 0) continue;
+            a[u] = __ldcs(kn + src[u]);
+            b[u] = __ldcs(vn + src[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+            if (slot[u] < 0) continue;
+            const int64_t page = p.narrow && slot[u] < (1ll << 31) ? (int64_t)p.div_p((uint32_t)slot[u])
+                                                                   : slot[u] / p.P;
+            if (page >= p.num_slots) { atomicMax(&g_error, kErrPage); continue; }
+            const int64_t dst = (page * p.stride_p + (slot[u] - page * p.P) * p.stride_t +
+                                 head[u] * p.stride_h) / elts + in_row[u];
+            k[dst] = a[u];
+            v[dst] = b[u];
+        }
     }
 }
 
@@ -258,14 +319,15 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t st) {
     for (const void* ptr : {(const void*)p.k, (const void*)p.v, p.k_new, p.v_new})
         vec = vec && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0;
     const int elts = vec ? 16 / eb : 1;
-    const int chunks = p.D / elts;
-    int64_t per = (1024 + p.Hkv * chunks - 1) / (p.Hkv * chunks);
-    const int64_t ctas = (p.T + per - 1) / per;
+    const int per_row = p.D / elts, per_token = p.Hkv * per_row;
+    const int each = kAppendThreads * kPieces;
+    const int tokens = per_token >= each ? 1 : each / per_token;
+    const int64_t ctas = (p.T + tokens - 1) / tokens;
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-    if (vec) append_kernel<uint4><<<(unsigned)ctas, 256, 0, st>>>(p, chunks, elts, per);
-    else if (eb == 2) append_kernel<uint16_t><<<(unsigned)ctas, 256, 0, st>>>(p, chunks, elts, per);
-    else append_kernel<uint32_t><<<(unsigned)ctas, 256, 0, st>>>(p, chunks, elts, per);
-    return counted(cudaGetLastError(), 1);
+    const FastDiv dt((uint32_t)per_token), dr((uint32_t)per_row);
+    if (vec) return launch(append_kernel<uint4>, ctas, kAppendThreads, st, p, dt, dr, per_token, per_row, elts, tokens);
+    if (eb == 2) return launch(append_kernel<uint16_t>, ctas, kAppendThreads, st, p, dt, dr, per_token, per_row, elts, tokens);
+    return launch(append_kernel<uint32_t>, ctas, kAppendThreads, st, p, dt, dr, per_token, per_row, elts, tokens);
 }
 
 cudaError_t read_table_error(int clear, int* code) {

@@ -24,7 +24,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import _lib
-from ._lib import KVLayout, Output, Query, check, dtype_code, require_cuda, stream_ptr
+from ._lib import KVLayout, Output, Query, check, dtype_code, require_cuda
 
 __all__ = [
     "RaggedTables",
@@ -45,27 +45,26 @@ class RaggedTables(NamedTuple):
     free_state: torch.Tensor     # [3] state of the ring of free pages
 
 
-class _on_device:
-    """Makes `device` current for a launch (nothing to do where it already is)."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _device_of(*tensors) -> int:
+    """Index of the CUDA device that all tensors (None aside) are on."""
+    index = tensors[0].get_device()     # -1 on the CPU
+    for t in tensors:
+        if t is not None and (t.get_device() != index or index < 0):
+            require_cuda(*tensors)
+            raise ValueError("tensors on different devices: "
+                             + ", ".join(sorted({str(t.device) for t in tensors if t is not None})))
+    return index
 
 
-def _same_device(first: torch.Tensor, *others):
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+def _launch(index: int, what: str, entry, *args):
+    """Calls a C entry with the current stream of device `index`, which is made current."""
+    _lib.ragged_devices.add(index)
+    if index == torch.cuda.current_device():
+        st = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            st = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    check(st, what)
 
 
 def _int64(name: str, t: torch.Tensor, dim: int):
@@ -118,17 +117,18 @@ def ragged_page_tables(
     ``page_table`` and ``free_ring`` are updated in place.  ``lengths`` and ``free_state`` are
     not unless ``inplace`` is set: the returned ones then ARE those tensors, updated.  Two
     calls on one ring must not overlap."""
-    require_cuda(lengths, new_lengths, page_table, free_ring, free_state)
-    for name, t, dim in (("lengths", lengths, 1), ("new_lengths", new_lengths, 1),
-                         ("page_table", page_table, 2), ("free_ring", free_ring, 1),
-                         ("free_state", free_state, 1)):
-        _int64(name, t, dim)
-    _same_device(lengths, new_lengths, page_table, free_ring, free_state)
+    index = _device_of(lengths, new_lengths, page_table, free_ring, free_state)
+    _int64("lengths", lengths, 1)
+    _int64("new_lengths", new_lengths, 1)
+    _int64("page_table", page_table, 2)
+    _int64("free_ring", free_ring, 1)
+    _int64("free_state", free_state, 1)
     R, W = page_table.shape
     if lengths.shape[0] != R or new_lengths.shape[0] != R:
         raise ValueError(f"lengths and new_lengths must be [{R}] like page_table's rows, got "
                          f"{tuple(lengths.shape)} and {tuple(new_lengths.shape)}")
-    if free_state.shape[0] != 3 or free_ring.shape[0] < 1:
+    slots = free_ring.shape[0]
+    if free_state.shape[0] != 3 or slots < 1:
         raise ValueError("free_state must be [3] and free_ring [num_slots], as ragged_free_ring makes them")
     if page_size < 1 or max_new_tokens < 0:
         raise ValueError(f"page_size {page_size} and max_new_tokens {max_new_tokens} must be positive")
@@ -137,22 +137,16 @@ def ragged_page_tables(
     _written("free_state", free_state)
     if inplace:
         _written("lengths", lengths)
-    dev = lengths.device
     n, m = lengths.contiguous(), new_lengths.contiguous()
-    out = torch.empty(R + 1 + 2 * max_new_tokens + (0 if inplace else R + 3), dtype=torch.int64,
-                      device=dev)
-    slots, positions, starts = out[:max_new_tokens], out[max_new_tokens: 2 * max_new_tokens], \
-        out[2 * max_new_tokens: 2 * max_new_tokens + R + 1]
-    after, state = (lengths, free_state) if inplace else (out[-R - 3: -3], out[-3:])
-    _lib.ragged_devices.add(dev.index)
-    with _on_device(dev):
-        st = _lib.load().rkv_ragged_page_tables(
+    slot_map, positions = n.new_empty(max_new_tokens), n.new_empty(max_new_tokens)
+    starts = n.new_empty(R + 1)
+    after, state = (lengths, free_state) if inplace else (n.new_empty(R), n.new_empty(3))
+    _launch(index, "rkv_ragged_page_tables", _lib.load().rkv_ragged_page_tables,
             n.data_ptr(), m.data_ptr(), R, page_size, page_table.data_ptr(), W, W,
-            free_ring.data_ptr(), free_ring.shape[0], free_state.data_ptr(), after.data_ptr(),
-            state.data_ptr(), slots.data_ptr(), positions.data_ptr(), max_new_tokens,
-            starts.data_ptr(), stream_ptr(dev))
-    check(st, "rkv_ragged_page_tables")
-    return RaggedTables(after, slots, positions, starts, state)
+            free_ring.data_ptr(), slots, free_state.data_ptr(), after.data_ptr(),
+            state.data_ptr(), slot_map.data_ptr(), positions.data_ptr(), max_new_tokens,
+            starts.data_ptr())
+    return RaggedTables(after, slot_map, positions, starts, state)
 
 
 def _pool_layout(key_pool, value_pool, batch, table, capacity) -> KVLayout:
@@ -185,9 +179,8 @@ def ragged_append(
 
     Negative slots are skipped (a padded tail); one past the pool is skipped and raised by
     ``check_device_errors``.  Rows of one slot must not repeat: either may be the one left."""
-    require_cuda(key, value, key_pool, value_pool, slot_map)
+    index = _device_of(key, value, key_pool, value_pool, slot_map)
     _int64("slot_map", slot_map, 1)
-    _same_device(key, value, key_pool, value_pool, slot_map)
     lay = _pool_layout(key_pool, value_pool, 0, None, 0)
     T = slot_map.shape[0]
     if key.shape != (T, lay.num_kv_heads, lay.head_dim) or value.shape != key.shape:
@@ -202,12 +195,8 @@ def ragged_append(
     if k.stride() != v.stride():
         k, v = k.contiguous(), v.contiguous()
     slots = slot_map.contiguous()
-    dev = key.device
-    _lib.ragged_devices.add(dev.index)
-    with _on_device(dev):
-        st = _lib.load().rkv_ragged_append(lay, k.data_ptr(), v.data_ptr(), k.stride(0),
-                                           k.stride(1), T, slots.data_ptr(), stream_ptr(dev))
-    check(st, "rkv_ragged_append")
+    _launch(index, "rkv_ragged_append", _lib.load().rkv_ragged_append, lay, k.data_ptr(),
+            v.data_ptr(), k.stride(0), k.stride(1), T, slots.data_ptr())
 
 
 def ragged_decode_attention(
@@ -234,7 +223,7 @@ def ragged_decode_attention(
 
     Lengths outside [0, W * P] and page ids outside the pool are kept inside them and raised by
     ``check_device_errors``; ``validate`` checks them on the host first (one device sync)."""
-    require_cuda(query, key_pool, value_pool, page_table, lengths, starts, out)
+    index = _device_of(query, key_pool, value_pool, page_table, lengths, starts, out)
     if query.dim() != 4:
         raise ValueError(f"query must be [B, H, 1, D], got {tuple(query.shape)}")
     B, H, q_len, D = query.shape
@@ -243,9 +232,8 @@ def ragged_decode_attention(
     _int64("lengths", lengths, 1)
     if starts is not None:
         _int64("starts", starts, 1)
-    _same_device(query, key_pool, value_pool, page_table, lengths, starts, out)
     table = page_table if page_table.stride(1) == 1 else page_table.contiguous()
-    W = table.shape[1]
+    rows, W = table.shape
     lay = _pool_layout(key_pool, value_pool, B, table, W * key_pool.shape[2])
     if lay.head_dim != D:
         raise ValueError(f"the pool's head_dim {lay.head_dim} is not the query's {D}")
@@ -253,41 +241,39 @@ def ragged_decode_attention(
         raise ValueError(f"num_heads {H} is not a multiple of num_kv_heads {lay.num_kv_heads}")
     if query.dtype != key_pool.dtype:
         raise TypeError(f"query {query.dtype} and pool {key_pool.dtype} must share a dtype")
-    if table.shape[0] != B or lengths.shape[0] != B or (starts is not None and starts.shape[0] != B):
+    if rows != B or lengths.shape[0] != B or (starts is not None and starts.shape[0] != B):
         raise ValueError(f"page_table, lengths and starts must have one row per request ({B})")
     if scale is not None and not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if out is None:
-        out = torch.empty(B, H, 1, D, dtype=query.dtype, device=query.device)
+        out = query.new_empty((B, H, 1, D))
     elif out.shape != query.shape or out.dtype != query.dtype or out.stride(3) != 1:
         raise ValueError("out must have the query's shape and dtype, with contiguous rows")
     elif B and out.data_ptr() == query.data_ptr():
         raise ValueError("out must not be the query")
-    dev = query.device
-    lse = torch.empty(B, H, dtype=torch.float32, device=dev) if return_lse else None
+    lse = query.new_empty((B, H), dtype=torch.float32) if return_lse else None
     if B == 0:
         return (out, lse) if return_lse else out
-    # rows of 16-byte steps, as the tensor-core kernels read them
-    q, step = query, 16 // query.element_size()
-    if q.stride(3) != 1 or q.stride(0) % step or q.stride(1) % step or q.data_ptr() & 15:
-        q = torch.empty(B, H, 1, D, dtype=q.dtype, device=dev).copy_(query)
+    # rows of 16-byte steps, as the vector kernels read them
+    q, (sb, sh, st, sd), step = query, query.stride(), 16 // query.element_size()
+    if sd != 1 or sb % step or sh % step or q.data_ptr() & 15:
+        q = query.new_empty((B, H, 1, D)).copy_(query)
+        sb, sh, st, _ = q.stride()
     n = lengths.contiguous()
     first = starts.contiguous() if starts is not None else None
     if validate:
         _validate(table, n, lay)
-    qs = Query(q.data_ptr(), lay.dtype, H, 1, q.stride(0), q.stride(1), q.stride(2))
-    os_ = Output(out.data_ptr(), lay.dtype, 0, out.stride(0), out.stride(1), out.stride(2))
+    qs = Query(q.data_ptr(), lay.dtype, H, 1, sb, sh, st)
+    sb, sh, st, _ = out.stride()
+    os_ = Output(out.data_ptr(), lay.dtype, 0, sb, sh, st)
     lib = _lib.load()
     nbytes = lib.rkv_ragged_decode_attention_workspace_size(qs, lay)
-    _lib.ragged_devices.add(dev.index)
-    with _on_device(dev):
-        # of the caching allocator, so that each call and each captured graph has its own
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        st = lib.rkv_ragged_decode_attention(
-            qs, lay, n.data_ptr(), first.data_ptr() if first is not None else None,
-            float(scale) if scale is not None else 0.0, os_,
-            lse.data_ptr() if lse is not None else None, ws.data_ptr(), nbytes, stream_ptr(dev))
-    check(st, "rkv_ragged_decode_attention")
+    # of the caching allocator, so that each call and each captured graph has its own
+    ws = query.new_empty(nbytes, dtype=torch.uint8)
+    _launch(index, "rkv_ragged_decode_attention", lib.rkv_ragged_decode_attention, qs, lay,
+            n.data_ptr(), first.data_ptr() if first is not None else None,
+            scale if scale is not None else 0.0, os_, lse.data_ptr() if lse is not None else None,
+            ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
