@@ -32,7 +32,7 @@ namespace ragged {
 static __device__ int g_error;
 
 constexpr int kCtas = 148;      // one persistent CTA per SM
-constexpr int kMostWarps = 8;   // warps per CTA of any kernel here (16 at most: join_parts)
+constexpr int kMostWarps = 8;   // warps per CTA of any kernel here
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -212,6 +212,8 @@ struct Left {
     int64_t rest;           // tiles of the last segment behind the run
 };
 
+constexpr int kJoinRows = 2;
+
 __device__ __forceinline__ float4 lds_float4(uint32_t at, bool on) {
     float4 v;
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
@@ -225,14 +227,16 @@ __device__ __forceinline__ float4 lds_float4(uint32_t at, bool on) {
 
 // Joins the parts of a CTA's warps.  In the order of the warps, a tail, or the first head, starts
 // a chain, the heads behind it belong to the same segment, and one that ends closes it.  A warp
-// takes a row of a chain: lane v weighs the part of warp v, and the lanes add the row up, four
-// elements each.  parts: two places of `place` floats per warp, `stride` floats apart.
+// takes kJoinRows rows of a chain at a time: lane 8 y + v weighs row y of the part of warp v, and
+// the lanes add the rows up, four elements each.
+// parts: two places of `place` floats per warp, `stride` floats apart.
 template <int NW, int HG, int DT>
 __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r, const Workspace& ws,
                                            const Left* left, float* parts, int stride, int place, int groups) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = p.Hq / p.Hkv;
     const int c = blockIdx.x;
+    static_assert(NW <= 8 && HG % kJoinRows == 0, "lanes of a task");
     const bool in = lane < NW;
     const unsigned heads = __ballot_sync(0xffffffffu, in && left[lane].head);
     const unsigned tails = __ballot_sync(0xffffffffu, in && left[lane].tail);
@@ -259,61 +263,78 @@ __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r,
         const int hq0 = h * G + gi * HG, ng = min(HG, G - gi * HG);
         const bool whole = i > 0 && closed;
         const Part to = ws.cta(c, i > 0);
-        int row = turn;
+        constexpr int R = kJoinRows;
+        int task = turn;
 #pragma unroll 1
-        for (; row < ng; row += NW) {
-            const bool mine = members >> lane & 1;
-            const Part own{parts + (mine ? lane : w) * stride + (mine && second >> lane & 1 ? place : 0), HG, p.D};
-            const float t = mine ? own.top(row) : -INFINITY;
-            float top = t, sum = mine ? own.sum(row) : 0.f;
+        for (; task * R < ng; task += NW) {
+            const int row0 = task * R, v = lane & 7;
+            const bool mine = members >> v & 1;
+            const int own_row = row0 + (R == 1 ? 0 : lane >> 3 & (R - 1));
+            const Part own{parts + (mine ? v : w) * stride + (mine && second >> v & 1 ? place : 0), HG, p.D};
+            const float t = mine ? own.top(own_row) : -INFINITY;
+            float top = t, sum = mine ? own.sum(own_row) : 0.f;
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const float weight = mine ? sm100::ex2(t - (top == -INFINITY ? 0.f : top)) : 0.f;
             if (mine) sum *= weight;
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            top = __shfl_sync(0xffffffffu, top, 0);
-            sum = __shfl_sync(0xffffffffu, sum, 0);
-            const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-            if (lane == 0) {
-                if (!whole) { to.top(row) = top; to.sum(row) = sum; }
-                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + row] = lse_of(top, sum);
+            for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (v == 0 && lane < 8 * R && own_row < ng) {
+                if (!whole) { to.top(own_row) = top; to.sum(own_row) = sum; }
+                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + own_row] = lse_of(top, sum);
             }
-            const uint32_t from = sm100::smem_u32(Part{parts, HG, p.D}.acc(row));
+            const float inverse = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            const uint32_t from = sm100::smem_u32(Part{parts, HG, p.D}.acc(row0));
 #pragma unroll 1
             for (int d = lane * 4; d - lane * 4 < p.D; d += 128) {
-                float o[4] = {0.f, 0.f, 0.f, 0.f};
-                const bool all = p.D % 4 == 0;
-                if (all) {
+                float o[R][4];
 #pragma unroll
-                    for (int v = 0; v < NW; ++v) {
-                        const float a = __shfl_sync(0xffffffffu, weight, v);
-                        const float4 f = lds_float4(from + (v * stride + (second >> v & 1 ? place : 0) + d) * 4,
-                                                    (members >> v & 1) && d < p.D);
-                        o[0] = fmaf(f.x, a, o[0]); o[1] = fmaf(f.y, a, o[1]);
-                        o[2] = fmaf(f.z, a, o[2]); o[3] = fmaf(f.w, a, o[3]);
+                for (int y = 0; y < R; ++y)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[y][x] = 0.f;
+                if (p.D % 4 == 0) {
+#pragma unroll
+                    for (int u = 0; u < NW; ++u) {
+                        const bool on = (members >> u & 1) && d < p.D;
+                        const uint32_t at = from + (u * stride + (second >> u & 1 ? place : 0) + d) * 4;
+#pragma unroll
+                        for (int y = 0; y < R; ++y) {
+                            const float a = __shfl_sync(0xffffffffu, weight, y * 8 + u);
+                            const float4 f = lds_float4(at + y * (p.D + 4) * 4, on);
+                            o[y][0] = fmaf(f.x, a, o[y][0]); o[y][1] = fmaf(f.y, a, o[y][1]);
+                            o[y][2] = fmaf(f.z, a, o[y][2]); o[y][3] = fmaf(f.w, a, o[y][3]);
+                        }
                     }
                 } else {
 #pragma unroll 1
-                    for (int v = 0; v < NW; ++v) {
-                        const float a = __shfl_sync(0xffffffffu, weight, v);
-                        if (!(members >> v & 1)) continue;
-                        const float* f = Part{parts + v * stride + (second >> v & 1 ? place : 0), HG, p.D}.acc(row);
+                    for (int u = 0; u < NW; ++u) {
+                        const Part part{parts + u * stride + (second >> u & 1 ? place : 0), HG, p.D};
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            if (d + x < p.D) o[x] = fmaf(f[d + x], a, o[x]);
+                        for (int y = 0; y < R; ++y) {
+                            const float a = __shfl_sync(0xffffffffu, weight, y * 8 + u);
+                            if (!(members >> u & 1)) continue;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                if (d + x < p.D) o[y][x] = fmaf(part.acc(row0 + y)[d + x], a, o[y][x]);
+                        }
                     }
                 }
-                const int64_t at = (int64_t)b * p.o_stride_b + (int64_t)(hq0 + row) * p.o_stride_h + d;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    if (d + x >= p.D) break;
-                    if (whole) store_elt(p.out, at + x, DT < 0 ? p.dtype : DT, o[x] * scale);
-                    else to.acc(row)[d + x] = o[x];
+                for (int y = 0; y < R; ++y) {
+                    const int row = row0 + y;
+                    const float scale = __shfl_sync(0xffffffffu, inverse, y * 8);
+                    if (row >= ng) break;
+                    const int64_t at = (int64_t)b * p.o_stride_b + (int64_t)(hq0 + row) * p.o_stride_h + d;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        if (d + x >= p.D) break;
+                        if (whole) store_elt(p.out, at + x, DT < 0 ? p.dtype : DT, o[y][x] * scale);
+                        else to.acc(row)[d + x] = o[y][x];
+                    }
                 }
             }
         }
-        turn = row - ng;
+        turn = task - (ng + R - 1) / R;
         turn = turn >= NW ? turn - NW : turn;
         if (i > 0 && !closed && threadIdx.x == 0) {
             const int z = 31 - __clz(members);      // last warp of the chain
@@ -1143,17 +1164,17 @@ decode_any_kernel(DecodeParams p, int groups) {
 
 // ------------------------------------------------------------------------------------------
 // CTA (c, row): row `row` of the segment that goes on behind the run of decode CTA c, if one
-// does: its part there and one part of each CTA behind, at most kCtas in all.  A thread per part
-// weighs it, and warp w sums the parts w, w + kMergeWarps, ..., whose sums are added in order.
+// does: its part there and one part of each CTA behind, at most kCtas in all.  The threads weigh
+// the parts, and warp w sums the parts w, w + kMergeWarps, ..., whose sums are added in order.
 // All of it is waiting for memory, so the first kMergeAhead parts of each warp are on their way
 // before the weights are known.
 // ------------------------------------------------------------------------------------------
-constexpr int kMergeWarps = 8, kMergeAhead = 5;
-static_assert(kMergeWarps * 32 >= kCtas && kMergeWarps * 32 >= kMaxHeadDim, "a thread per part");
+constexpr int kMergeWarps = 4, kMergeAhead = 10, kMergeThreads = kMergeWarps * 32;
+static_assert(2 * kMergeThreads >= kCtas, "a thread weighs up to two parts");
 
 __global__ void __launch_bounds__(kMergeWarps * 32)
 merge_kernel(DecodeParams p, int groups, int HG) {
-    __shared__ float s_weight[kMergeWarps * 32], s_top[kMergeWarps], s_sum[kMergeWarps];
+    __shared__ float s_weight[2 * kMergeThreads], s_top[kMergeWarps], s_sum[kMergeWarps];
     __shared__ float s_acc[kMergeWarps][kMaxHeadDim];
     sm100::grid_launch_dependents();
     sm100::grid_dependency_wait();
@@ -1168,8 +1189,12 @@ merge_kernel(DecodeParams p, int groups, int HG) {
     // part 0 is the open one of CTA c, part i > 0 the first of CTA c + i
     const float* parts = ws.cta(c, 0).at;
     auto at = [&](int i) { return parts + (2 * i + (i == 0)) * ws.stride; };
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (tid < n) ml = *reinterpret_cast<const float2*>(&Part{const_cast<float*>(at(tid)), HG, p.D}.top(row));
+    float2 ml[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = tid + k * kMergeThreads;
+        ml[k] = i < n ? *reinterpret_cast<const float2*>(at(i) + 2 * row) : make_float2(-INFINITY, 0.f);
+    }
     const int skip = 2 * HG + row * (p.D + 4) + lane;
     float ahead[kMergeAhead][4];
 #pragma unroll
@@ -1178,16 +1203,20 @@ merge_kernel(DecodeParams p, int groups, int HG) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) ahead[k][x] = lane + 32 * x < p.D ? f[32 * x] : 0.f;
     }
-    float top = ml.x;
+    float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) s_top[warp] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_top[w]);
-    const float weight = sm100::ex2(ml.x - (top == -INFINITY ? 0.f : top));
-    s_weight[tid] = weight;
-    float sum = tid < n ? ml.y * weight : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float weight = sm100::ex2(ml[k].x - (top == -INFINITY ? 0.f : top));
+        s_weight[tid + k * kMergeThreads] = weight;
+        if (tid + k * kMergeThreads < n) sum += ml[k].y * weight;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
@@ -1218,11 +1247,11 @@ merge_kernel(DecodeParams p, int groups, int HG) {
     }
     __syncthreads();
     const int hq = h * G + g0 + row;
-    if (tid < p.D) {
+    for (int d = tid; d < p.D; d += kMergeThreads) {
         float o = 0.f;
 #pragma unroll
-        for (int w = 0; w < kMergeWarps; ++w) o += s_acc[w][tid];
-        store_elt(p.out, (int64_t)open.x * p.o_stride_b + (int64_t)hq * p.o_stride_h + tid, p.dtype,
+        for (int w = 0; w < kMergeWarps; ++w) o += s_acc[w][d];
+        store_elt(p.out, (int64_t)open.x * p.o_stride_b + (int64_t)hq * p.o_stride_h + d, p.dtype,
                   sum == 0.f ? 0.f : o / sum);
     }
     if (p.lse && tid == 0) p.lse[(int64_t)open.x * p.Hq + hq] = lse_of(top, sum);
