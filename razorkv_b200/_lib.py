@@ -11,6 +11,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "librazorkv_b200.so")
+RAGGED_PATH = os.path.join(_HERE, "_lib", "_ragged.so")
 
 c_i64 = ctypes.c_int64
 c_i32 = ctypes.c_int32
@@ -179,8 +180,33 @@ DEVICE_ERRORS = {
        "length or the free ring's state was out of range (no page was taken or given back)",
 }
 
-# Devices on which a ragged operator has run: their error words are read by check_device_errors.
-ragged_devices = set()
+_ragged = None
+
+
+def ragged():
+    """The ragged operators' binding (_ragged.so), bound to the library's entries."""
+    global _ragged
+    if _ragged is None:
+        lib = load()
+        if not os.path.exists(RAGGED_PATH):
+            raise ImportError(f"{RAGGED_PATH} is missing; build it with `python -m razorkv_b200.build`")
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_file_location
+        spec = spec_from_file_location("_ragged", RAGGED_PATH,
+                                       loader=ExtensionFileLoader("_ragged", RAGGED_PATH))
+        module = module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(RazorKVError, *(ctypes.cast(getattr(lib, name), c_vp).value for name in (
+            "rkv_ragged_page_tables", "rkv_ragged_append", "rkv_ragged_decode_attention",
+            "rkv_ragged_decode_attention_workspace_size", "rkv_status_string")))
+        _ragged = module
+    return _ragged
+
+
+def ragged_devices():
+    """Devices on which a ragged operator has run: their error words are worth reading."""
+    mask = _ragged.devices() if _ragged is not None else 0
+    return [i for i in range(64) if mask >> i & 1]
 
 
 def ragged_error(device_index: int, clear: bool = True) -> int:

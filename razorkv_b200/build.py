@@ -1,4 +1,5 @@
-"""Builds librazorkv_b200.so (the C-ABI CUDA library) in-tree for sm_100a.
+"""Builds librazorkv_b200.so (the C-ABI CUDA library) in-tree for sm_100a, and _ragged.so, the
+ragged operators' binding of it to torch tensors.
 
     python -m razorkv_b200.build            # incremental
     python -m razorkv_b200.build --force    # rebuild every object
@@ -18,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(HERE, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "librazorkv_b200.so")
+BINDING_PATH = os.path.join(LIB_DIR, "_ragged.so")
 
 SOURCES = ["rkv_capi.cu", "rkv_generic.cu", "rkv_decode_sm100.cu", "rkv_noalloc.cu",
            "rkv_ragged.cu", "rkv_ragged_tables.cu", "rkv_ragged_decode.cu"]
@@ -71,7 +73,29 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link of librazorkv_b200.so failed")
+    _build_binding(force)
     return LIB_PATH
+
+
+def _build_binding(force: bool):
+    src = os.path.join(CSRC, "rkv_ragged_binding.cpp")
+    header = os.path.join(ROOT, "include", "razorkv_b200.h")
+    if not force and not _stale(BINDING_PATH, [src, header, __file__]):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    dirs = include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in dirs), src, "-o", BINDING_PATH, *(f"-L{d}" for d in library_paths()),
+           "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("build of _ragged.so failed")
 
 
 if __name__ == "__main__":

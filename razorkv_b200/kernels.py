@@ -97,7 +97,7 @@ class Workspace:
                     continue
                 flags = cls._retired.pop(dev, []) if clear else cls._retired.get(dev, [])
                 codes += [int(f.item()) for f in flags if int(f.item())]
-            for dev in sorted(_lib.ragged_devices):
+            for dev in _lib.ragged_devices():
                 if want is None or dev == want:
                     codes += [c for c in [_lib.ragged_error(dev, clear)] if c]
         if codes:

@@ -6,23 +6,7 @@ import pytest
 import torch
 
 import razorkv_b200 as R
-from razorkv_b200 import _lib, ragged
-
-
-@pytest.fixture
-def no_device(monkeypatch):
-    """The operators' argument checks on CPU tensors: the device check is lifted, and a call
-    that passes them all ends before the library."""
-    class Reached(Exception):
-        pass
-
-    def reached(*a):
-        raise Reached
-
-    monkeypatch.setattr(ragged, "_device_of", lambda *t: 0)
-    monkeypatch.setattr(ragged._lib, "load", reached)
-    monkeypatch.setattr(ragged._lib, "ragged_devices", set())
-    return Reached
+from razorkv_b200 import _lib
 
 
 def _tables(**changes):
@@ -48,18 +32,12 @@ def _attend(**changes):
     return R.ragged_decode_attention(**a)
 
 
-def test_valid_calls_pass_the_checks(no_device):
-    for call in (_tables, _append, _attend):
-        with pytest.raises(no_device):
-            call()
-    with pytest.raises(no_device):
-        _attend(starts=torch.tensor([0, 3]), scale=0.5, out=torch.zeros(2, 4, 1, 8))
-    with pytest.raises(no_device):
-        _tables(inplace=True)
-
-
-def test_cpu_tensors_are_refused():
-    for call in (_tables, _append, _attend):
+def test_valid_calls_end_at_the_device():
+    """Nothing but the device is wrong with these (tensors on the CPU: it is looked at last)."""
+    for call in (_tables, _append, _attend, lambda: _tables(inplace=True),
+                 lambda: _attend(starts=torch.tensor([0, 3]), scale=0.5, return_lse=True,
+                                 out=torch.zeros(2, 4, 1, 8)),
+                 lambda: _attend(starts=torch.tensor([0, 3]), scale=2, validate=True)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
 
@@ -73,13 +51,16 @@ def test_cpu_tensors_are_refused():
     (dict(free_state=torch.tensor([0, 9])), ValueError),
     (dict(free_ring=torch.zeros(0, dtype=torch.int64)), ValueError),
     (dict(page_size=0), ValueError),
+    (dict(page_size=1.5), TypeError),
+    (dict(page_size=1 << 70), TypeError),
+    (dict(free_ring=None), TypeError),
     (dict(max_new_tokens=-1), ValueError),
     (dict(page_table=torch.zeros(5, 2, dtype=torch.int64).t()), ValueError),
     (dict(page_table=torch.zeros(1, 5, dtype=torch.int64).expand(2, 5)), ValueError),
     (dict(free_ring=torch.arange(18)[::2]), ValueError),
     (dict(lengths=torch.tensor([3, 9, 0, 9])[::2], inplace=True), ValueError),
 ])
-def test_tables_refusals(no_device, changes, error):
+def test_tables_refusals(changes, error):
     with pytest.raises(error):
         _tables(**changes)
 
@@ -101,7 +82,7 @@ def test_tables_refusals(no_device, changes, error):
           key_pool=torch.zeros(5, 2, 4, 8, dtype=torch.float64),
           value_pool=torch.zeros(5, 2, 4, 8, dtype=torch.float64)), TypeError),
 ])
-def test_append_refusals(no_device, changes, error):
+def test_append_refusals(changes, error):
     with pytest.raises(error):
         _append(**changes)
 
@@ -119,6 +100,10 @@ def test_append_refusals(no_device, changes, error):
     (dict(starts=torch.tensor([1])), ValueError),
     (dict(starts=torch.tensor([1., 2.])), TypeError),
     (dict(scale=0.0), ValueError),
+    (dict(scale=1e-60), ValueError),
+    (dict(scale=1e60), ValueError),
+    (dict(scale="x"), TypeError),
+    (dict(query=None), TypeError),
     (dict(scale=-1.0), ValueError),
     (dict(scale=float("nan")), ValueError),
     (dict(scale=float("inf")), ValueError),
@@ -126,18 +111,18 @@ def test_append_refusals(no_device, changes, error):
     (dict(out=torch.zeros(2, 4, 1, 8, dtype=torch.float16)), ValueError),
     (dict(value_pool=torch.zeros(5, 2, 8, 8)), ValueError),
 ])
-def test_attend_refusals(no_device, changes, error):
+def test_attend_refusals(changes, error):
     with pytest.raises(error):
         _attend(**changes)
 
 
-def test_attend_refuses_its_query_as_output(no_device):
+def test_attend_refuses_its_query_as_output():
     q = torch.zeros(2, 4, 1, 8)
     with pytest.raises(ValueError, match="query"):
         _attend(query=q, out=q)
 
 
-def test_validation_names_bad_lengths_and_pages(no_device):
+def test_validation_names_bad_lengths_and_pages():
     with pytest.raises(IndexError, match="lengths"):
         _attend(lengths=torch.tensor([1, 13]), validate=True)
     with pytest.raises(IndexError, match="lengths"):
@@ -145,7 +130,7 @@ def test_validation_names_bad_lengths_and_pages(no_device):
     bad = torch.tensor([[0, 9, 9], [4, 5, 0]])
     with pytest.raises(IndexError, match="page_table"):
         _attend(page_table=bad, lengths=torch.tensor([4, 7]), validate=True)
-    with pytest.raises(no_device):   # entries past a request's tokens are not looked at
+    with pytest.raises(RuntimeError, match="CUDA"):   # entries past a request's tokens are not looked at
         _attend(page_table=bad, lengths=torch.tensor([4, 4]), validate=True)
 
 
@@ -216,7 +201,7 @@ def test_check_reads_only_devices_that_ran_a_ragged_operator(monkeypatch):
     seen = []
     monkeypatch.setattr(Workspace, "_pool", {})
     monkeypatch.setattr(Workspace, "_retired", {})
-    monkeypatch.setattr(_lib, "ragged_devices", {1})
+    monkeypatch.setattr(_lib, "ragged_devices", lambda: [1])
     monkeypatch.setattr(_lib, "ragged_error", lambda dev, clear: seen.append((dev, clear)) or 3)
     with pytest.raises(_lib.DeviceError) as e:
         check_device_errors()
