@@ -65,6 +65,17 @@ __device__ __forceinline__ int64_t tiles_of(int64_t first, int64_t last) {
 // tiles of 16; 255 of up to 509: 26.3 us with 1, 28.4 with 2 tiles of 32.)
 __host__ __device__ constexpr int over_of(int tile_tokens) { return tile_tokens <= 16 ? 2 : 1; }
 
+// Segments of so few tiles are not split between warps, or between CTAs: the boundary between two
+// runs moves to the nearer end of its segment.  Where no segment can have more tiles than are
+// split between CTAs, merge_kernel is not launched.
+struct Whole {
+    int warp, cta;
+};
+constexpr int kWarpFew = 4, kWarpMany = 8, kCtaFew = 4, kCtaMany = 16;
+constexpr Whole whole_tiles(int64_t segments, int64_t warps) {
+    return 2 * segments >= warps ? Whole{kWarpMany, kCtaMany} : Whole{kWarpFew, kCtaFew};
+}
+
 // a / b of non-negative numbers, the 32-bit way where it can be
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
@@ -123,7 +134,7 @@ struct Runs {
 };
 
 template <int TT, int NW>
-__device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_tile) {
+__device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_tile, Whole whole) {
     constexpr int T = NW * 32;
     __shared__ int64_t s_sums[NW];
     __shared__ int64_t s_before[T];
@@ -157,40 +168,59 @@ __device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_til
     __syncthreads();
     r.ctas = max((int64_t)1, min((int64_t)gridDim.x, divide(r.total, NW)));
     if (blockIdx.x >= r.ctas) return r;
+    // Of each boundary: the first tile behind it, the tiles before that one, and the unit at which
+    // the boundary has come to lie.  Even lanes look for the start of a run, odd ones for its end;
+    // first of the CTA's run (if its boundaries may move), then of the warp's share of it.
     const Deal deal(r.total, r.ctas);
-    const int64_t cta0 = deal.start(blockIdx.x);
-    r.cta1 = deal.start(blockIdx.x + 1);
-    const Deal own(r.cta1 - cta0, NW);
-    // even lanes look for the start of the warp's run, odd ones for its end
-    const int64_t target = cta0 + own.start(warp + (lane & 1));
-    int i = 0;
-#pragma unroll
-    for (int step = 512; step > 0; step >>= 1)
-        if (i + step < T && s_before[i + step] <= target) i += step;
-    int64_t at = s_before[i];
-    int b = i * per;
-    int64_t units = 0;
-    if (b < p.B) {
-        range_of(p, b, &f, &l);
-        r.tiles = tiles_of<TT>(f, l);
-        units = (r.tiles + kOver) * per_tile;
-    }
+    int64_t target = deal.start(blockIdx.x + (lane & 1)), tiles_before = 0;
+    int b = 0;
 #pragma unroll 1
-    for (int k = 1; k < per && b + 1 < p.B && target >= at + units; ++k) {
-        at += units;
-        ++b;
+    for (int pass = whole.cta > whole.warp ? 0 : 1; pass < 2; ++pass) {
+        if (pass == 1) {
+            const int64_t cta0 = __shfl_sync(0xffffffffu, target, 0);
+            r.cta1 = __shfl_sync(0xffffffffu, target, 1);
+            target = cta0 + Deal(r.cta1 - cta0, NW).start(warp + (lane & 1));
+        }
+        const int upto = pass == 0 ? whole.cta : whole.warp;
+        if (target >= r.total) {
+            tiles_before = r.total - kOver * per_tile * p.B;
+            continue;
+        }
+        int i = 0;
+#pragma unroll
+        for (int step = 512; step > 0; step >>= 1)
+            if (i + step < T && s_before[i + step] <= target) i += step;
+        int64_t at = s_before[i];
+        b = i * per;
         range_of(p, b, &f, &l);
         r.tiles = tiles_of<TT>(f, l);
-        units = (r.tiles + kOver) * per_tile;
-    }
-    // tiles before the target: those of the requests before, and of this one
-    int64_t tiles_before;
-    if (target >= r.total) {
-        tiles_before = r.total - kOver * per_tile * p.B;
-    } else {
-        r.seg = (int)divide(target - at, r.tiles + kOver);
-        r.tile = max((int64_t)0, target - at - r.seg * (r.tiles + kOver) - kOver);
+        int64_t units = (r.tiles + kOver) * per_tile;
+#pragma unroll 1
+        while (target >= at + units) {      // (only where a thread has summed several requests)
+            at += units;
+            range_of(p, ++b, &f, &l);
+            r.tiles = tiles_of<TT>(f, l);
+            units = (r.tiles + kOver) * per_tile;
+        }
+        const int64_t length = r.tiles + kOver;
+        r.seg = (int)divide(target - at, length);
+        const int64_t seg_at = at + r.seg * length, in_seg = target - seg_at;
+        r.tile = max((int64_t)0, in_seg - kOver);
+        if (r.tiles <= upto) {
+            r.tile = 2 * in_seg > length ? r.tiles : 0;
+            target = seg_at + (r.tile ? length : 0);
+        }
         tiles_before = at - kOver * per_tile * b + r.seg * r.tiles + r.tile;
+        if (r.tile == r.tiles) {        // the start of the next segment
+            r.tile = 0;
+            if (++r.seg == per_tile) {
+                r.seg = 0;
+                if (++b < p.B) {
+                    range_of(p, b, &f, &l);
+                    r.tiles = tiles_of<TT>(f, l);
+                }
+            }
+        }
     }
     r.count = __shfl_sync(0xffffffffu, tiles_before, 1) - __shfl_sync(0xffffffffu, tiles_before, 0);
     r.b = __shfl_sync(0xffffffffu, b, 0);
@@ -430,7 +460,7 @@ constexpr float kSlack = 8.f;
 // kWhole: pages hold a multiple of 16 tokens, so 16 rows have one page.
 template <bool kBf16, int DP, int NH, int TT, int NW, int STAGES, bool kWhole>
 __global__ void __launch_bounds__(NW * 32, 1)
-decode_tc_kernel(DecodeParams p, int groups) {
+decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(TT % 16 == 0 && TT <= 32 && DP % 64 == 0 && (NH == 1 || NH == 2), "shape");
     extern __shared__ __align__(128) char smem[];
@@ -447,7 +477,7 @@ decode_tc_kernel(DecodeParams p, int groups) {
     const int G = p.Hq / p.Hkv;
     const Workspace ws(p, MH);
 
-    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups);
+    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups, upto);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
@@ -787,7 +817,7 @@ struct F32Shape {
 
 template <int DP, int HG, int TT, int NW, int STAGES>
 __global__ void __launch_bounds__(NW * 32, 1)
-decode_f32_kernel(DecodeParams p, int groups) {
+decode_f32_kernel(DecodeParams p, int groups, Whole upto) {
     using Shape = F32Shape<DP, HG, TT, NW, STAGES>;
     static_assert(HG % 4 == 0 && DP % 64 == 0 && (TT == 8 || TT == 16), "shape");
     extern __shared__ __align__(128) char smem[];
@@ -804,7 +834,7 @@ decode_f32_kernel(DecodeParams p, int groups) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = p.Hq / p.Hkv;
     const Workspace ws(p, HG);
-    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups);
+    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups, upto);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
@@ -1046,7 +1076,7 @@ decode_f32_kernel(DecodeParams p, int groups) {
 constexpr int kAnyTile = 16, kAnyWarps = 8, kAnyHeads = 4;
 
 __global__ void __launch_bounds__(kAnyWarps * 32)
-decode_any_kernel(DecodeParams p, int groups) {
+decode_any_kernel(DecodeParams p, int groups, Whole upto) {
     constexpr int HG = kAnyHeads, kPlace = Part::floats(HG, kMaxHeadDim);
     extern __shared__ __align__(128) char smem[];
     __shared__ Left left[kAnyWarps];
@@ -1054,7 +1084,7 @@ decode_any_kernel(DecodeParams p, int groups) {
     sm100::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Workspace ws(p, HG);
-    const Runs runs = find_runs<kAnyTile, kAnyWarps>(p, (int64_t)p.Hkv * groups);
+    const Runs runs = find_runs<kAnyTile, kAnyWarps>(p, (int64_t)p.Hkv * groups, upto);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
@@ -1270,10 +1300,10 @@ bool tc_ok(const DecodeParams& p) {
     return p.o_stride_b % 2 == 0 && p.o_stride_h % 2 == 0 && !(reinterpret_cast<uintptr_t>(p.out) & 3);
 }
 
-// A decode kernel and its merge, each launched so that its start overlaps the end of the kernel
+// A decode kernel and its merge (where there can be something to join), each launched so that its start overlaps the end of the kernel
 // before it (both wait for that kernel's results first).
-template <void (*kernel)(DecodeParams, int)>
-cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, cudaStream_t st) {
+template <void (*kernel)(DecodeParams, int, Whole)>
+cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, int TT, cudaStream_t st) {
     const int groups = (p.Hq / p.Hkv + HG - 1) / HG;
     // the kernel's shared memory is set once per device (a setting of the function, not of a call)
     static std::atomic<uint64_t> set{0};
@@ -1295,8 +1325,11 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, cu
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = counted(cudaLaunchKernelEx(&cfg, kernel, p, groups), 1);
-    if (e != cudaSuccess) return e;
+    const Whole upto = whole_tiles((int64_t)p.B * p.Hkv * groups, (int64_t)kCtas * threads / 32);
+    e = counted(cudaLaunchKernelEx(&cfg, kernel, p, groups, upto), 1);
+    // (a range of tokens that does not start at a tile's first reaches into one tile more)
+    const int64_t most = (p.W * p.P + TT - 1) / TT + (p.starts ? 1 : 0);
+    if (e != cudaSuccess || most <= upto.cta) return e;
     cfg.gridDim = dim3(kCtas, HG);
     cfg.blockDim = dim3(kMergeWarps * 32);
     cfg.dynamicSmemBytes = 0;
@@ -1308,7 +1341,7 @@ cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
     constexpr int TT = DP <= 128 ? 32 : 16, NW = DP <= 64 ? 8 : DP <= 128 ? 4 : 6 - NH, STAGES = 2;
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 4096, "shared memory");
-    return launch_pair<decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>>(NW * 32, Shape::kSmem, p, NH * 8, st);
+    return launch_pair<decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>>(NW * 32, Shape::kSmem, p, NH * 8, TT, st);
 }
 
 template <int DP, int NH>
@@ -1339,7 +1372,7 @@ cudaError_t launch_f32(const DecodeParams& p, cudaStream_t st) {
     constexpr int TT = DP <= 64 ? 16 : 8, NW = DP <= 128 ? 10 - HG / 2 : 5 - HG / 4, STAGES = 2;
     using Shape = F32Shape<DP, HG, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 8192, "shared memory");
-    return launch_pair<decode_f32_kernel<DP, HG, TT, NW, STAGES>>(NW * 32, Shape::kSmem, p, HG, st);
+    return launch_pair<decode_f32_kernel<DP, HG, TT, NW, STAGES>>(NW * 32, Shape::kSmem, p, HG, TT, st);
 }
 
 template <int DP>
@@ -1361,7 +1394,7 @@ cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
         return launch_f32_heads<256>(p, st);
     }
     if (!tc_ok(p)) return launch_pair<decode_any_kernel>(kAnyWarps * 32,
-                                       kAnyWarps * 2 * Part::floats(kAnyHeads, kMaxHeadDim) * 4, p, kAnyHeads, st);
+                                       kAnyWarps * 2 * Part::floats(kAnyHeads, kMaxHeadDim) * 4, p, kAnyHeads, kAnyTile, st);
     if (p.D <= 64) return launch_tc_heads<64>(p, st);
     if (p.D <= 128) return launch_tc_heads<128>(p, st);
     return launch_tc_heads<256>(p, st);
