@@ -811,7 +811,10 @@ struct F32Shape {
     static constexpr int kLpt = 32 / TT;                // lanes per token
     static constexpr int kPitch = DP * 4 + 16 * kLpt;   // 8 lanes at a time read 128 different bytes
     static constexpr int kPlane = TT * kPitch;
-    static constexpr int kStage = 2 * kPlane + HG * kPitch;
+    // Queries come with the first tile of their segment; with 8 heads they would take the room of
+    // two warps, and are read when the segment begins (8 requests of 9155 tokens, 4 kv heads x 128: 88 and 77 us).
+    static constexpr bool kQInRing = HG <= 4;
+    static constexpr int kStage = 2 * kPlane + (kQInRing ? HG * kPitch : 0);
     static constexpr int kSmem = NW * (STAGES * kStage + HG * kPitch);
 };
 
@@ -860,7 +863,7 @@ decode_f32_kernel(DecodeParams p, int groups, Whole upto) {
             if (ahead > 0) {
                 const int t0 = put.token0();
                 const uint32_t dst = ring + stage * Shape::kStage;
-                if (with_q) {
+                if (Shape::kQInRing && with_q) {
                     const int g0 = put.gi * HG, ng = min(HG, G - g0);
                     const char* src = static_cast<const char*>(p.q) +
                                       ((int64_t)put.b * p.q_stride_b + (int64_t)(put.h * G + g0) * p.q_stride_h) * 4;
@@ -927,8 +930,22 @@ decode_f32_kernel(DecodeParams p, int groups, Whole upto) {
             __syncwarp();
             const uint32_t at = stage * Shape::kStage;
             if (get.tile == tile_in) {
-                for (int x = lane; x < HG * Shape::kPitch / 16; x += 32)
-                    reinterpret_cast<uint4*>(q_own)[x] = sm100::lds128(ring + at + 2 * Shape::kPlane + x * 16);
+                if constexpr (Shape::kQInRing) {
+                    for (int x = lane; x < HG * Shape::kPitch / 16; x += 32)
+                        reinterpret_cast<uint4*>(q_own)[x] = sm100::lds128(ring + at + 2 * Shape::kPlane + x * 16);
+                } else {
+                    const int g0 = get.gi * HG, ng = min(HG, G - g0);
+                    const float* src = static_cast<const float*>(p.q) + (int64_t)get.b * p.q_stride_b +
+                                       (int64_t)(get.h * G + g0) * p.q_stride_h;
+#pragma unroll
+                    for (int j = 0; j < HG * kChunks / 32; ++j) {
+                        const int x = lane + 32 * j, r = x / kChunks, c = x % kChunks;
+                        const float4 v = r < ng && c * 4 < p.D
+                                             ? *reinterpret_cast<const float4*>(src + r * p.q_stride_h + c * 4)
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+                        *reinterpret_cast<float4*>(q_own + r * (Shape::kPitch / 4) + c * 4) = v;
+                    }
+                }
                 __syncwarp();
             }
             uint64_t s2[HG];
@@ -1369,7 +1386,9 @@ bool f32_ok(const DecodeParams& p) {
 
 template <int DP, int HG>
 cudaError_t launch_f32(const DecodeParams& p, cudaStream_t st) {
-    constexpr int TT = DP <= 64 ? 16 : 8, NW = DP <= 128 ? 10 - HG / 2 : 5 - HG / 4, STAGES = 2;
+    // (8 heads x 128: 67 us with four warps and tiles of 16 tokens, 77 with eight and 8)
+    constexpr bool kWide = DP == 128 && HG == 8;
+    constexpr int TT = DP <= 64 || kWide ? 16 : 8, NW = DP <= 128 && !kWide ? 8 : 4, STAGES = 2;
     using Shape = F32Shape<DP, HG, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 8192, "shared memory");
     return launch_pair<decode_f32_kernel<DP, HG, TT, NW, STAGES>>(NW * 32, Shape::kSmem, p, HG, TT, st);
