@@ -1355,7 +1355,7 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, in
 
 template <bool kBf16, int DP, int NH, bool kWhole>
 cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
-    constexpr int TT = DP <= 128 ? 32 : 16, NW = DP <= 64 ? 8 : DP <= 128 ? 4 : 6 - NH, STAGES = 2;
+    constexpr int TT = DP <= 128 ? 32 : 16, NW = DP <= 64 ? 8 : 4, STAGES = 2;
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 4096, "shared memory");
     return launch_pair<decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>>(NW * 32, Shape::kSmem, p, NH * 8, TT, st);
