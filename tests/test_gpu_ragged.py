@@ -607,3 +607,33 @@ def test_launches_are_counted():
     before = lib.rkv_launch_count()
     R.ragged_decode_attention(q, kp, vp, table, n)
     assert lib.rkv_launch_count() > before
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,P,lengths", [
+    (torch.bfloat16, 32, 8, 128, 16, [30011, 5, 0, 17000, 64, 9000]),
+    (torch.float16, 28, 4, 128, 16, [90001, 1, 33]),
+    (torch.bfloat16, 16, 16, 64, 16, [20000, 20001, 7, 19999]),
+    (torch.float16, 32, 2, 128, 64, [60000, 300, 41000]),
+    (torch.bfloat16, 12, 4, 256, 5, [20000, 15, 20003]),
+    (torch.float32, 8, 4, 128, 16, [20000, 3, 30001]),
+])
+def test_attention_large(dtype, Hq, Hkv, D, P, lengths):
+    """Long requests beside short ones; they repeat bit for bit, and as a graph whose lengths change."""
+    case = _pool_case(lengths, Hq, Hkv, D, P, dtype, seed=sum(lengths))
+    out, lse = (t.clone() for t in _compare(case))
+    q, kp, vp, table, n, s = case
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        again = R.ragged_decode_attention(q, kp, vp, table, n, return_lse=True)
+    for _ in range(5):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    # the same tables with little in them
+    few = torch.tensor([min(x, 40 + 3 * i) for i, x in enumerate(lengths)], device="cuda")
+    _compare((q, kp, vp, table, few, s))
+    n.copy_(few)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again[0], R.ragged_decode_attention(q, kp, vp, table, few))
+    check_device_errors()
