@@ -13,6 +13,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <optional>
@@ -180,7 +181,8 @@ PyObject* tables(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (page < 1 || most < 0)
             refuse(PyExc_ValueError, "page_size " + std::to_string(page) + " and max_new_tokens " +
                                          std::to_string(most) + " must be positive");
-        want_written(table, "page_table");
+        if (table.numel() && (table.stride(1) != 1 || (R > 1 && table.stride(0) < W)))
+            refuse(PyExc_ValueError, "page_table is updated in place: its rows must be contiguous and apart");
         want_written(ring, "free_ring");
         want_written(state, "free_state");
         if (inplace) want_written(lengths, "lengths");
@@ -192,7 +194,8 @@ PyObject* tables(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         at::Tensor starts = at::empty({R + 1}, options);
         at::Tensor after = inplace ? lengths : at::empty({R}, options);
         at::Tensor state_after = inplace ? state : at::empty({3}, options);
-        launch.check(g_tables(n.data_ptr<int64_t>(), m.data_ptr<int64_t>(), R, page, table.data_ptr<int64_t>(), W, W,
+        launch.check(g_tables(n.data_ptr<int64_t>(), m.data_ptr<int64_t>(), R, page, table.data_ptr<int64_t>(),
+                              std::max(table.stride(0), W), W,
                               ring.data_ptr<int64_t>(), ring.size(0), state.data_ptr<int64_t>(),
                               after.data_ptr<int64_t>(), state_after.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
                               positions.data_ptr<int64_t>(), most, starts.data_ptr<int64_t>(), launch.stream),

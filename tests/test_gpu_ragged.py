@@ -412,6 +412,12 @@ def test_tables_repeat_and_corners():
     _check_tables(n, m, table, ring, state, 4, 12)
     _check_tables(a.lengths, a.lengths, table, ring, a.free_state, 4, 0)
     _check_tables(a.lengths, torch.zeros_like(n), table, ring, a.free_state, 4, 0)
+    # columns of a wider table, and a single row of one
+    wide = torch.full((5, 9), 9, dtype=torch.int64, device=dev)
+    c = _check_tables(n, m, wide[:3, 2:6], ring, state, 4, 13)
+    assert torch.equal(c.slot_map, a.slot_map) and torch.equal(wide[:3, 2:6][0, :1], table[0, :1])
+    assert bool((wide[3:] == 9).all()) and bool((wide[:, :2] == 9).all()) and bool((wide[:, 6:] == 9).all())
+    _check_tables(n[:1], m[:1], wide[4:5, :4], ring, state, 4, 4)
     # no requests
     none = torch.zeros(0, dtype=torch.int64, device=dev)
     t = _check_tables(none, none, torch.zeros(0, 4, dtype=torch.int64, device=dev), ring, state, 4, 5)
