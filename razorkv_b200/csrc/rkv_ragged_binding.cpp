@@ -153,6 +153,15 @@ bool want_args(Py_ssize_t got, Py_ssize_t want) {
     return false;
 }
 
+// n elements of a contiguous tensor, from `offset` on, as a tensor of their own on its storage (a
+// third of the time that an allocation or a view through the dispatcher takes).
+at::Tensor carve(const at::Tensor& from, int64_t offset, int64_t n) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(from.storage()), from.key_set(), from.dtype());
+    impl->set_storage_offset(offset);
+    impl->set_sizes_contiguous({n});
+    return at::Tensor(std::move(impl));
+}
+
 // tables(lengths, new_lengths, page_table, free_ring, free_state, page_size, max_new_tokens, inplace)
 //   -> (lengths, slot_map, positions, token_starts, free_state)
 PyObject* tables(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -190,10 +199,12 @@ PyObject* tables(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const Launch launch(index);
         const at::Tensor n = lengths.contiguous(), m = wanted.contiguous();
         const auto options = n.options().requires_grad(false);
-        at::Tensor slots = at::empty({most}, options), positions = at::empty({most}, options);
-        at::Tensor starts = at::empty({R + 1}, options);
-        at::Tensor after = inplace ? lengths : at::empty({R}, options);
-        at::Tensor state_after = inplace ? state : at::empty({3}, options);
+        // per token, and per request (which a caller may keep longer)
+        const at::Tensor per_token = at::empty({2 * most}, options), per_request = at::empty({2 * R + 4}, options);
+        at::Tensor slots = carve(per_token, 0, most), positions = carve(per_token, most, most);
+        at::Tensor starts = carve(per_request, 0, R + 1);
+        at::Tensor after = inplace ? lengths : carve(per_request, R + 1, R);
+        at::Tensor state_after = inplace ? state : carve(per_request, 2 * R + 1, 3);
         launch.check(g_tables(n.data_ptr<int64_t>(), m.data_ptr<int64_t>(), R, page, table.data_ptr<int64_t>(),
                               std::max(table.stride(0), W), W,
                               ring.data_ptr<int64_t>(), ring.size(0), state.data_ptr<int64_t>(),

@@ -67,7 +67,11 @@ __host__ __device__ constexpr int over_of(int tile_tokens) { return tile_tokens 
 
 // Segments of so few tiles are not split between warps, or between CTAs: the boundary between two
 // runs moves to the nearer end of its segment.  Where no segment can have more tiles than are
-// split between CTAs, merge_kernel is not launched.
+// split between CTAs, merge_kernel is not launched.  With at least half as many segments as
+// warps, moving boundaries costs less balance than parts cost joins: 64 requests of 250 tokens
+// (8 kv heads x 128, 8 tiles) take 16.3 us whole and 22.8 split, 64 of 500 28.9 and 34.6, but 8 of
+// 250 11.9 whole and 10.3 split.  Limits of 12 and 16 tiles for warps cost requests of mixed
+// lengths more than they gave (255 of 1 to 509 tokens, 16 heads x 64: 24.5 us, 27 and 27.6).
 struct Whole {
     int warp, cta;
 };
@@ -414,13 +418,18 @@ struct Walk {
 // takes half the registers.  P^T gets from the accumulator's layout to the operand's by an 8x8
 // transpose in registers.
 // Rounding P to 16 bits alone would add an error as large as the output's own rounding, so P
-// goes in as hi + lo, both 16-bit.  The base of the power is a maximum seen so far that is
+// goes in as hi + lo, both 16-bit (with 16 heads, where products cost most, 19.7 us instead of
+// 19.1 for 16 requests of up to 16384 tokens).  The base of the power is a maximum seen so far that is
 // only renewed when a logit exceeds it by more than 2^kSlack, which saves the reduction over
 // lanes on most tiles; weights are then at most 2^kSlack instead of 1.  In fp16 they are scaled
 // by 2^kBias besides, so that small ones stay in fp16's normal range; that scale is part of the
 // base and cancels.
 // Rows outside the request's range are filled with zeros without being read: what the pool
 // holds there (NaN included) never enters a product.
+// Bound by memory: 8 requests of 32768 tokens (8 x 128, bf16) take 181 us, 5.9 TB/s of K and V,
+// 1 of 131072 (4 x 128) 53 us, 5.1 TB/s; about 7 us of a call are not: its launches, the sums over
+// the requests, the first tile's way, the joins.  Tensor pipes stay below a tenth of their rate up
+// to 8 heads per kv head; 16 heads reach 4.8 TB/s.
 // ------------------------------------------------------------------------------------------
 // 16 bytes, or zeros without a read
 __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool on) {
@@ -457,7 +466,8 @@ struct TcShape {
 
 constexpr float kSlack = 8.f;
 
-// kWhole: pages hold a multiple of 16 tokens, so 16 rows have one page.
+// kWhole: pages hold a multiple of 16 tokens, so 16 rows have one page (8 requests of 18310 tokens,
+// 96 dims and 16 heads on each of 4: 67 us, 71 with a page per row).
 template <bool kBf16, int DP, int NH, int TT, int NW, int STAGES, bool kWhole>
 __global__ void __launch_bounds__(NW * 32, 1)
 decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
@@ -803,8 +813,8 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
 // fp32.  The same rings, with fp32 arithmetic (a product of tensor cores would round K and V to
 // fewer bits).  For the logits, LPT lanes share a token and read its row a quarter (half) each,
 // the queries come as broadcasts; for the output, a lane has DP / 32 dims of every head.  Both
-// halves are fused multiply-adds on pairs.  At HG heads per kv head that is 4 HG operations for
-// each 8 bytes read, a quarter of what the SMs could do while memory delivers them at HG = 8.
+// halves are fused multiply-adds on pairs.  Up to 4 heads per kv head memory is the bound (8
+// requests of 9155 tokens, 4 kv heads x 128: 54 us, 5.5 TB/s), with 8 the instructions are (67 us).
 // ------------------------------------------------------------------------------------------
 template <int DP, int HG, int TT, int NW, int STAGES>
 struct F32Shape {
@@ -1355,7 +1365,13 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, in
 
 template <bool kBf16, int DP, int NH, bool kWhole>
 cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
-    constexpr int TT = DP <= 128 ? 32 : 16, NW = DP <= 64 ? 8 : 4, STAGES = 2;
+    // Tiles of 16 KB of K and V a warp and two of them in its ring: 128 KB on their way per SM, where
+    // 64 KB do not fill the memory (8 requests of 32768 tokens, 8 x 128: 207 us, 181 with 128 KB, 187
+    // with 256).  Four warps leave fewer parts to join than eight (1 request of 131072 tokens, 4 x 128:
+    // 53 and 57 us; 64 of 250, 8 x 128: 16.3 and 22.1), but 16 heads at a time are more work per tile
+    // than one warp per scheduler does in time (64 requests of 500 tokens, 2 x 128: 23.1 and 21.4).
+    constexpr bool kWide = DP == 128 && NH == 2;
+    constexpr int TT = DP <= 128 && !kWide ? 32 : 16, NW = DP <= 64 || kWide ? 8 : 4, STAGES = 2;
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 4096, "shared memory");
     return launch_pair<decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>>(NW * 32, Shape::kSmem, p, NH * 8, TT, st);
