@@ -57,6 +57,7 @@ struct DecodeParams {
     void* out; int64_t o_stride_b, o_stride_h; float* lse;
     void* ws;
     FastDiv div_p;      // by P, where it is below 2^31
+    int narrow;         // units of work are 31-bit numbers
 };
 
 cudaError_t launch_tables(const TableParams& p, cudaStream_t st);

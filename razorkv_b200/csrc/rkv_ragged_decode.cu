@@ -80,23 +80,23 @@ constexpr Whole whole_tiles(int64_t segments, int64_t warps) {
     return 2 * segments >= warps ? Whole{kWarpMany, kCtaMany} : Whole{kWarpFew, kCtaFew};
 }
 
-// a / b of non-negative numbers, the 32-bit way where it can be
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
+// a / b of non-negative numbers
+__device__ __forceinline__ int divide(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) { return a / b; }
 
 // n runs of as nearly equal length as may be, the longer ones first: with q = units / n and
 // x = units % n, run i starts at i q + min(i, x).
+template <typename I>
 struct Deal {
-    int64_t q, x;
-    __device__ __forceinline__ Deal(int64_t units, int64_t n) {
+    I q, x;
+    __device__ __forceinline__ Deal(I units, I n) {
         q = divide(units, n);
         x = units - q * n;
     }
-    __device__ __forceinline__ int64_t start(int64_t i) const { return i * q + min(i, x); }
+    __device__ __forceinline__ I start(I i) const { return i * q + min(i, x); }
     // the run that holds a unit
-    __device__ __forceinline__ int64_t of(int64_t unit) const {
-        const int64_t longer = x * (q + 1);
+    __device__ __forceinline__ I of(I unit) const {
+        const I longer = x * (q + 1);
         return unit < longer ? divide(unit, q + 1) : x + divide(unit - longer, q);
     }
 };
@@ -137,91 +137,94 @@ struct Runs {
     int64_t tile, tiles, first, last;   // and the request's tiles per segment, and its tokens
 };
 
-template <int TT, int NW>
-__device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_tile, Whole whole) {
+// Unit counts are 31-bit numbers wherever the page tables cannot hold more (p.narrow): this code
+// runs once and takes as long as it has instructions.
+template <typename I, int TT, int NW>
+__device__ __forceinline__ Runs find_runs_in(const DecodeParams& p, I per_tile, Whole whole, I* s_sums, I* s_before) {
     constexpr int T = NW * 32;
-    __shared__ int64_t s_sums[NW];
-    __shared__ int64_t s_before[T];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (p.B + T - 1) / T;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-    int64_t mine = 0, f = 0, l = 0;
+    I mine = 0;
+    int64_t f = 0, l = 0;
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
         range_of(p, b, &f, &l);
-        mine += (tiles_of<TT>(f, l) + over_of(TT)) * per_tile;
+        mine += ((I)tiles_of<TT>(f, l) + over_of(TT)) * per_tile;
     }
-    int64_t x = mine;
+    I x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        const I y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     if (lane == 31) s_sums[warp] = x;
     __syncthreads();
     constexpr int kOver = over_of(TT);
     Runs r{};
-    int64_t before = x - mine;
+    I before = x - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-        const int64_t y = s_sums[w];
+        const I y = s_sums[w];
         before += w < warp ? y : 0;
-        r.total += y;
+        total += y;
     }
     s_before[tid] = before;
     __syncthreads();
-    r.ctas = max((int64_t)1, min((int64_t)gridDim.x, divide(r.total, NW)));
-    if (blockIdx.x >= r.ctas) return r;
+    const I ctas = max((I)1, min((I)gridDim.x, divide(total, (I)NW)));
+    r.total = total;
+    r.ctas = ctas;
+    if ((I)blockIdx.x >= ctas) return r;
     // Of each boundary: the first tile behind it, the tiles before that one, and the unit at which
     // the boundary has come to lie.  Even lanes look for the start of a run, odd ones for its end;
     // first of the CTA's run (if its boundaries may move), then of the warp's share of it.
-    const Deal deal(r.total, r.ctas);
-    int64_t target = deal.start(blockIdx.x + (lane & 1)), tiles_before = 0;
+    const Deal<I> deal(total, ctas);
+    I target = deal.start((I)blockIdx.x + (lane & 1)), tiles_before = 0, tiles = 0, tile = 0;
     int b = 0;
 #pragma unroll 1
     for (int pass = whole.cta > whole.warp ? 0 : 1; pass < 2; ++pass) {
         if (pass == 1) {
-            const int64_t cta0 = __shfl_sync(0xffffffffu, target, 0);
-            r.cta1 = __shfl_sync(0xffffffffu, target, 1);
-            target = cta0 + Deal(r.cta1 - cta0, NW).start(warp + (lane & 1));
+            const I cta0 = __shfl_sync(0xffffffffu, target, 0), cta1 = __shfl_sync(0xffffffffu, target, 1);
+            r.cta1 = cta1;
+            target = cta0 + Deal<I>(cta1 - cta0, NW).start(warp + (lane & 1));
         }
         const int upto = pass == 0 ? whole.cta : whole.warp;
-        if (target >= r.total) {
-            tiles_before = r.total - kOver * per_tile * p.B;
+        if (target >= total) {
+            tiles_before = total - kOver * per_tile * p.B;
             continue;
         }
         int i = 0;
 #pragma unroll
         for (int step = 512; step > 0; step >>= 1)
             if (i + step < T && s_before[i + step] <= target) i += step;
-        int64_t at = s_before[i];
+        I at = s_before[i];
         b = i * per;
         range_of(p, b, &f, &l);
-        r.tiles = tiles_of<TT>(f, l);
-        int64_t units = (r.tiles + kOver) * per_tile;
+        tiles = (I)tiles_of<TT>(f, l);
+        I units = (tiles + kOver) * per_tile;
 #pragma unroll 1
         while (target >= at + units) {      // (only where a thread has summed several requests)
             at += units;
             range_of(p, ++b, &f, &l);
-            r.tiles = tiles_of<TT>(f, l);
-            units = (r.tiles + kOver) * per_tile;
+            tiles = (I)tiles_of<TT>(f, l);
+            units = (tiles + kOver) * per_tile;
         }
-        const int64_t length = r.tiles + kOver;
+        const I length = tiles + kOver;
         r.seg = (int)divide(target - at, length);
-        const int64_t seg_at = at + r.seg * length, in_seg = target - seg_at;
-        r.tile = max((int64_t)0, in_seg - kOver);
-        if (r.tiles <= upto) {
-            r.tile = 2 * in_seg > length ? r.tiles : 0;
-            target = seg_at + (r.tile ? length : 0);
+        const I seg_at = at + r.seg * length, in_seg = target - seg_at;
+        tile = max((I)0, in_seg - kOver);
+        if (tiles <= upto) {
+            tile = 2 * in_seg > length ? tiles : 0;
+            target = seg_at + (tile ? length : 0);
         }
-        tiles_before = at - kOver * per_tile * b + r.seg * r.tiles + r.tile;
-        if (r.tile == r.tiles) {        // the start of the next segment
-            r.tile = 0;
+        tiles_before = at - kOver * per_tile * b + r.seg * tiles + tile;
+        if (tile == tiles) {        // the start of the next segment
+            tile = 0;
             if (++r.seg == per_tile) {
                 r.seg = 0;
                 if (++b < p.B) {
                     range_of(p, b, &f, &l);
-                    r.tiles = tiles_of<TT>(f, l);
+                    tiles = (I)tiles_of<TT>(f, l);
                 }
             }
         }
@@ -229,11 +232,20 @@ __device__ __forceinline__ Runs find_runs(const DecodeParams& p, int64_t per_til
     r.count = __shfl_sync(0xffffffffu, tiles_before, 1) - __shfl_sync(0xffffffffu, tiles_before, 0);
     r.b = __shfl_sync(0xffffffffu, b, 0);
     r.seg = __shfl_sync(0xffffffffu, r.seg, 0);
-    r.tile = __shfl_sync(0xffffffffu, r.tile, 0);
-    r.tiles = __shfl_sync(0xffffffffu, r.tiles, 0);
+    r.tile = __shfl_sync(0xffffffffu, tile, 0);
+    r.tiles = __shfl_sync(0xffffffffu, tiles, 0);
     r.first = __shfl_sync(0xffffffffu, f, 0);
     r.last = __shfl_sync(0xffffffffu, l, 0);
     return r;
+}
+
+template <int TT, int NW>
+__device__ __forceinline__ Runs find_runs(const DecodeParams& p, int groups, Whole whole) {
+    __shared__ int64_t s_sums[NW], s_before[NW * 32];
+    const int per_tile = p.Hkv * groups;
+    if (p.narrow)
+        return find_runs_in<int, TT, NW>(p, per_tile, whole, reinterpret_cast<int*>(s_sums), reinterpret_cast<int*>(s_before));
+    return find_runs_in<int64_t, TT, NW>(p, per_tile, whole, s_sums, s_before);
 }
 
 // What a warp leaves for the join: the part of a segment that began before its run (`head`), and
@@ -373,7 +385,7 @@ __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r,
         if (i > 0 && !closed && threadIdx.x == 0) {
             const int z = 31 - __clz(members);      // last warp of the chain
             const int64_t last = r.cta1 + left[z].rest - 1;
-            ws.open[c] = make_int4(b, seg, (int)(Deal(r.total, r.ctas).of(last) - c), 0);
+            ws.open[c] = make_int4(b, seg, (int)(Deal<int64_t>(r.total, r.ctas).of(last) - c), 0);
         }
     }
 }
@@ -487,7 +499,7 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
     const int G = p.Hq / p.Hkv;
     const Workspace ws(p, MH);
 
-    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups, upto);
+    const Runs runs = find_runs<TT, NW>(p, groups, upto);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
@@ -847,7 +859,7 @@ decode_f32_kernel(DecodeParams p, int groups, Whole upto) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = p.Hq / p.Hkv;
     const Workspace ws(p, HG);
-    const Runs runs = find_runs<TT, NW>(p, (int64_t)p.Hkv * groups, upto);
+    const Runs runs = find_runs<TT, NW>(p, groups, upto);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
@@ -1111,7 +1123,7 @@ decode_any_kernel(DecodeParams p, int groups, Whole upto) {
     sm100::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Workspace ws(p, HG);
-    const Runs runs = find_runs<kAnyTile, kAnyWarps>(p, (int64_t)p.Hkv * groups, upto);
+    const Runs runs = find_runs<kAnyTile, kAnyWarps>(p, groups, upto);
     if (blockIdx.x >= runs.ctas) {
         if (threadIdx.x == 0) ws.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
@@ -1352,8 +1364,12 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, in
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    DecodeParams q = p;
+    // (units beyond the tiles of the table's capacity: one for a range that starts within a tile, one
+    // or two for the segment itself; doubled, for the search that moves boundaries)
+    q.narrow = (double)p.B * p.Hkv * groups * ((double)p.W * p.P / TT + 4) * 2 < 2147483647.0;
     const Whole upto = whole_tiles((int64_t)p.B * p.Hkv * groups, (int64_t)kCtas * threads / 32);
-    e = counted(cudaLaunchKernelEx(&cfg, kernel, p, groups, upto), 1);
+    e = counted(cudaLaunchKernelEx(&cfg, kernel, q, groups, upto), 1);
     // (a range of tokens that does not start at a tile's first reaches into one tile more)
     const int64_t most = (p.W * p.P + TT - 1) / TT + (p.starts ? 1 : 0);
     if (e != cudaSuccess || most <= upto.cta) return e;

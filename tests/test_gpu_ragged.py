@@ -266,6 +266,16 @@ def test_attention_device_errors():
     check_device_errors()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("width", [200, 32767, 32769])
+def test_attention_wide_tables(dtype, width):
+    """Tables whose capacity in tiles, or in tokens, is beyond 31 bits."""
+    case = _pool_case([70000, 131077, 3] + [0] * 59 + [65536, 1], 2, 1, 8, 65536, dtype, seed=11,
+                      width=width)
+    _compare(case)
+    check_device_errors()
+
+
 # ---- append -------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("T,Hkv,D,P,layout,offset", [
