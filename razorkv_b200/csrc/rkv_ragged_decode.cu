@@ -67,17 +67,26 @@ __host__ __device__ constexpr int over_of(int tile_tokens) { return tile_tokens 
 
 // Segments of so few tiles are not split between warps, or between CTAs: the boundary between two
 // runs moves to the nearer end of its segment.  Where no segment can have more tiles than are
-// split between CTAs, merge_kernel is not launched.  With at least half as many segments as
-// warps, moving boundaries costs less balance than parts cost joins: 64 requests of 250 tokens
-// (8 kv heads x 128, 8 tiles) take 16.3 us whole and 22.8 split, 64 of 500 28.9 and 34.6, but 8 of
-// 250 11.9 whole and 10.3 split.  Limits of 12 and 16 tiles for warps cost requests of mixed
+// split between CTAs, merge_kernel is not launched.
+// With at least half as many segments as warps, moving boundaries costs less balance than parts
+// cost joins: 64 requests of 250 tokens (8 kv heads x 128, 8 tiles) take 15.6 us whole and 22.8
+// split, 64 of 500 28.9 and 34.6; limits of 12 and 16 tiles for warps cost requests of mixed
 // lengths more than they gave (255 of 1 to 509 tokens, 16 heads x 64: 24.5 us, 27 and 27.6).
+// With fewer, a segment has a CTA to itself if `most`, the tiles that the page table has room for,
+// are at most two per warp: 8 requests of 250 tokens (8 heads x 128) take 8.5 us, 10.1 with a limit
+// of four tiles for both, 1 of 77 6.3 and 6.9, 1 of 256 8.1 and 8.9.  Up to four tiles per warp, 1
+// of 500 takes 10.8 us instead of 9.1; split between warps from two tiles on, not three, 1 of 64
+// takes 6.6 us instead of 6.0.  Where other segments may be longer, this keeps a CTA at what all
+// could share (5 requests of up to 9001 tokens in fp32, 4 heads x 64, windows of 1 to 5000: 11.9 us
+// instead of 10.6).
 struct Whole {
     int warp, cta;
 };
-constexpr int kWarpFew = 4, kWarpMany = 8, kCtaFew = 4, kCtaMany = 16;
-constexpr Whole whole_tiles(int64_t segments, int64_t warps) {
-    return 2 * segments >= warps ? Whole{kWarpMany, kCtaMany} : Whole{kWarpFew, kCtaFew};
+constexpr int kWarpShort = 2, kShortPerWarp = 2, kWarpFew = 4, kWarpMany = 8, kCtaMany = 16;
+constexpr Whole whole_tiles(int64_t segments, int64_t most, int warps_per_cta) {
+    if (2 * segments >= kCtas * warps_per_cta) return Whole{kWarpMany, kCtaMany};
+    if (most <= kShortPerWarp * warps_per_cta) return Whole{kWarpShort, kShortPerWarp * warps_per_cta};
+    return Whole{kWarpFew, kWarpFew};
 }
 
 // a / b of non-negative numbers
@@ -147,10 +156,13 @@ __device__ __forceinline__ Runs find_runs_in(const DecodeParams& p, I per_tile, 
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
     I mine = 0;
     int64_t f = 0, l = 0;
+    bool between = false;       // a segment that may be split between warps, but not between CTAs
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
         range_of(p, b, &f, &l);
-        mine += ((I)tiles_of<TT>(f, l) + over_of(TT)) * per_tile;
+        const I t = (I)tiles_of<TT>(f, l);
+        mine += (t + over_of(TT)) * per_tile;
+        between = between || (t > whole.warp && t <= whole.cta);
     }
     I x = mine;
 #pragma unroll
@@ -170,19 +182,20 @@ __device__ __forceinline__ Runs find_runs_in(const DecodeParams& p, I per_tile, 
         total += y;
     }
     s_before[tid] = before;
-    __syncthreads();
+    between = __syncthreads_or(between);
     const I ctas = max((I)1, min((I)gridDim.x, divide(total, (I)NW)));
     r.total = total;
     r.ctas = ctas;
     if ((I)blockIdx.x >= ctas) return r;
     // Of each boundary: the first tile behind it, the tiles before that one, and the unit at which
     // the boundary has come to lie.  Even lanes look for the start of a run, odd ones for its end;
-    // first of the CTA's run (if its boundaries may move), then of the warp's share of it.
+    // first of the CTA's run (if its boundaries may move where warps' do not), then of the warp's
+    // share of it.
     const Deal<I> deal(total, ctas);
     I target = deal.start((I)blockIdx.x + (lane & 1)), tiles_before = 0, tiles = 0, tile = 0;
     int b = 0;
 #pragma unroll 1
-    for (int pass = whole.cta > whole.warp ? 0 : 1; pass < 2; ++pass) {
+    for (int pass = between ? 0 : 1; pass < 2; ++pass) {
         if (pass == 1) {
             const I cta0 = __shfl_sync(0xffffffffu, target, 0), cta1 = __shfl_sync(0xffffffffu, target, 1);
             r.cta1 = cta1;
@@ -1368,10 +1381,10 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, in
     // (units beyond the tiles of the table's capacity: one for a range that starts within a tile, one
     // or two for the segment itself; doubled, for the search that moves boundaries)
     q.narrow = (double)p.B * p.Hkv * groups * ((double)p.W * p.P / TT + 4) * 2 < 2147483647.0;
-    const Whole upto = whole_tiles((int64_t)p.B * p.Hkv * groups, (int64_t)kCtas * threads / 32);
-    e = counted(cudaLaunchKernelEx(&cfg, kernel, q, groups, upto), 1);
     // (a range of tokens that does not start at a tile's first reaches into one tile more)
     const int64_t most = (p.W * p.P + TT - 1) / TT + (p.starts ? 1 : 0);
+    const Whole upto = whole_tiles((int64_t)p.B * p.Hkv * groups, most, threads / 32);
+    e = counted(cudaLaunchKernelEx(&cfg, kernel, q, groups, upto), 1);
     if (e != cudaSuccess || most <= upto.cta) return e;
     cfg.gridDim = dim3(kCtas, HG);
     cfg.blockDim = dim3(kMergeWarps * 32);
@@ -1384,7 +1397,7 @@ cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
     // Tiles of 16 KB of K and V a warp and two of them in its ring: 128 KB on their way per SM, where
     // 64 KB do not fill the memory (8 requests of 32768 tokens, 8 x 128: 207 us, 181 with 128 KB, 187
     // with 256).  Four warps leave fewer parts to join than eight (1 request of 131072 tokens, 4 x 128:
-    // 53 and 57 us; 64 of 250, 8 x 128: 16.3 and 22.1), but 16 heads at a time are more work per tile
+    // 53 and 57 us; 64 of 250, 8 x 128: 15.6 and 22.1), but 16 heads at a time are more work per tile
     // than one warp per scheduler does in time (64 requests of 500 tokens, 2 x 128: 23.1 and 21.4).
     constexpr bool kWide = DP == 128 && NH == 2;
     constexpr int TT = DP <= 128 && !kWide ? 32 : 16, NW = DP <= 64 || kWide ? 8 : 4, STAGES = 2;

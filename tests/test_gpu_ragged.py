@@ -266,6 +266,19 @@ def test_attention_device_errors():
     check_device_errors()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (16, 1, 128), (12, 3, 64), (6, 2, 200), (3, 1, 33)])
+@pytest.mark.parametrize("lengths", [[256], [129, 1, 0, 65], [250] * 9, [17, 64, 33, 100, 32, 256, 255],
+                                     [128, 120, 113, 40, 16]])
+def test_attention_tables_of_few_tiles(dtype, Hq, Hkv, D, lengths):
+    # tables with room for 4 to 33 tiles, from full to a token long, of calls whose segments are few
+    P = 32
+    for starts in (None, [max(0, n - 37 * (i + 1)) for i, n in enumerate(lengths)]):
+        for width in (-(-max(lengths) // P), 8, 9):
+            if width * P >= max(lengths):
+                _compare(_pool_case(lengths, Hq, Hkv, D, P, dtype, seed=11, starts=starts, width=width))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("width", [200, 32767, 32769])
 def test_attention_wide_tables(dtype, width):
