@@ -485,7 +485,8 @@ int rkv_ragged_append(const rkv_kv_layout* pool, const void* k_new, const void* 
 /* out[b, h] = softmax(q . k * scale) . v over the tokens starts[b] <= t < lengths[b] of request b
  * (starts == NULL: from the first), and lse[b * Hq + h] = log sum exp(q . k * scale) (natural,
  * fp32; may be NULL).  A request without such a token gives zeros and -inf, and what the pool
- * holds outside the tokens (NaN included) has no effect.  pool->batch is the number of
+ * holds outside the tokens (NaN included) has no effect; an infinite element of V in one of them
+ * makes its column infinite, or NaN where both signs meet.  pool->batch is the number of
  * requests and pool->num_tokens the table's capacity, pt_width * P.  scale == 0 selects
  * 1/sqrt(D).  q, pool and out share a dtype; q_len is 1.  A length outside [0, capacity] is
  * read as the nearer bound with error 3, a page id outside the pool as page 0 with error 2. */

@@ -17,6 +17,7 @@
 // at either end of the CTA's run; those go to the workspace, and merge_kernel joins them.  Parts
 // are joined in the order of the tokens, so results do not depend on timing, and nothing in the
 // workspace has to be set before the call.
+#include <float.h>
 #include <math.h>
 
 #include <atomic>
@@ -273,6 +274,10 @@ struct Left {
 
 constexpr int kJoinRows = 2;
 
+// What a part weighs whose maximum lies `down` below the largest one (exponents of two).  Never
+// zero: an infinity of V in a part stays one, however little the part weighs.
+__device__ __forceinline__ float part_weight(float down) { return fmaxf(sm100::ex2(down), FLT_MIN); }
+
 __device__ __forceinline__ float4 lds_float4(uint32_t at, bool on) {
     float4 v;
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
@@ -334,7 +339,7 @@ __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r,
             float top = t, sum = mine ? own.sum(own_row) : 0.f;
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float weight = mine ? sm100::ex2(t - (top == -INFINITY ? 0.f : top)) : 0.f;
+            const float weight = mine ? part_weight(t - (top == -INFINITY ? 0.f : top)) : 0.f;
             if (mine) sum *= weight;
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -490,6 +495,36 @@ struct TcShape {
 };
 
 constexpr float kSlack = 8.f;
+
+// Sums of the infinite and NaN elements of V over the tokens [t0, t1) of a request, for dims
+// 8 i + lane / 4 (zero where a column has none): what such a column of the output is, whatever the
+// (positive) weights are.  The products give NaN for it, since the low half of a weight may be zero
+// or negative.  Read again from the pool, by calls of such values only (the check costs 0.1 us of one
+// short request's 6.5, 0.4 us of 16 requests of up to 16384 tokens, 16 heads on each of 2 x 128).  The
+// four lanes of a dim share the tokens.
+template <bool kBf16, int DP>
+__device__ __noinline__ void odd_columns(float (&sum)[DP / 8], const void* v, const int64_t* table, int64_t num_slots,
+                                         int64_t P, int64_t stride_p, int64_t stride_t, int t0, int t1, int D) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) sum[i] = 0.f;
+    for (int64_t t = (int64_t)t0 + (lane & 3); t < t1; t += 4) {
+        const int64_t j = t / P;
+        int64_t page = table[j];
+        if (page < 0 || page >= num_slots) page = 0;
+        const int64_t row = page * stride_p + (t - j * P) * stride_t + (lane >> 2);
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            const float x = i * 8 < D ? load_elt(v, row + i * 8, kBf16 ? RKV_BF16 : RKV_F16) : 0.f;
+            sum[i] += isfinite(x) ? 0.f : x;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+    }
+}
 
 // kWhole: pages hold a multiple of 16 tokens, so 16 rows have one page (8 requests of 18310 tokens,
 // 96 dims and 16 heads on each of 4: 67 us, 71 with a page per row).
@@ -768,14 +803,44 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
                 }
                 const Part part = last ? Part{places, MH, p.D}
                                        : ws.warp((int64_t)blockIdx.x * NW + warp);
+                float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int n = 0; n < NH; ++n) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float sum = l[n][x];
-                        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-                        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-                        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
+                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
+                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
+                    }
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) zero[x] = fmaf(o[d][n][x], 0.f, zero[x]);
+                }
+                bool odd = false;       // an infinity or NaN, and weights that are none
+#pragma unroll
+                for (int n = 0; n < NH; ++n) odd = odd || l[n][0] > 0.f || l[n][1] > 0.f;
+                odd = odd && (zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.f;
+                if (__any_sync(0xffffffffu, odd)) {
+                    float sum[DP / 8];
+                    const int from = max(get.first, (int)(((uint32_t)get.first / TT + tile_in) * TT));
+                    odd_columns<kBf16, DP>(sum, static_cast<const char*>(p.v) + (int64_t)h * p.stride_h * 2,
+                                           p.table + (int64_t)get.b * p.table_stride, p.num_slots, p.P, p.stride_p,
+                                           p.stride_t, from, min(get.last, t0 + TT), p.D);
+#pragma unroll
+                    for (int n = 0; n < NH; ++n)
+#pragma unroll
+                        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                if (l[n][x & 1] > 0.f && isnan(o[d][n][x]) && sum[2 * d + x / 2] != 0.f)
+                                    o[d][n][x] = sum[2 * d + x / 2];
+                }
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float sum = l[n][x];
                         const int row = 8 * n + c2 + x;
                         const float b = limit[n][x] == -INFINITY ? -INFINITY : base[n][x];
                         if (g == 0 && row < ng) {
@@ -1295,7 +1360,7 @@ merge_kernel(DecodeParams p, int groups, int HG) {
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const float weight = sm100::ex2(ml[k].x - (top == -INFINITY ? 0.f : top));
+        const float weight = part_weight(ml[k].x - (top == -INFINITY ? 0.f : top));
         s_weight[tid + k * kMergeThreads] = weight;
         if (tid + k * kMergeThreads < n) sum += ml[k].y * weight;
     }

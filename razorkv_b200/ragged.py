@@ -119,7 +119,9 @@ def ragged_decode_attention(
     row ``t % P`` of page ``page_table[b, t // P]``.  Returns [B, H, 1, D] in the query's dtype
     (in ``out`` where given), and with ``return_lse`` also log sum exp(scale * q . k) as fp32
     [B, H].  A request without such a token (a padded batch) gives zeros and -inf, and what the
-    pool holds elsewhere has no effect.  ``scale`` defaults to 1 / sqrt(D).
+    pool holds elsewhere has no effect; infinities and NaN in attended rows take the formula's
+    way into the output (an infinite element of V makes its column infinite, or NaN where both
+    signs meet).  ``scale`` defaults to 1 / sqrt(D).
 
     Lengths outside [0, W * P] and page ids outside the pool are kept inside them and raised by
     ``check_device_errors``; ``validate`` checks them on the host first (one device sync)."""
