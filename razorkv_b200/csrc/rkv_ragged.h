@@ -54,6 +54,7 @@ struct DecodeParams {
     const int64_t* lengths; const int64_t* starts;
     int B, Hq, Hkv, D, dtype;
     float scale;
+    float bias;         // the kernel's weights are 2^bias times exp(scale * (q . k - base))
     void* out; int64_t o_stride_b, o_stride_h; float* lse;
     void* ws;
     FastDiv div_p;      // by P, where it is below 2^31

@@ -3,7 +3,10 @@
 //   o[b, h] = sum_t w_t v_t / sum_t w_t,  w_t = exp(scale q[b, h] . k_t),
 //   t in [start_b, len_b), k_t and v_t rows of kv head h / (Hq / Hkv)
 //
-// in one pass over K and V with a running maximum (in the exponent of two) and sum.
+// in one pass over K and V with a running maximum of q . k and sum.  A weight is the power of
+// scale * (q . k - maximum), the difference taken first: the maximum's own exponent is then exact
+// however large the logits are, where the difference of two rounded products is off by up to half a
+// step of the larger (32 at 1e9, beyond what a weight can hold).
 //
 // Work is cut into units of TT tokens of one (request, kv head, group of query heads): a
 // segment is all units of one such triple, and the units of all segments in a row are dealt out
@@ -37,9 +40,11 @@ constexpr int kMostWarps = 8;   // warps per CTA of any kernel here
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Natural logarithm of sum * 2^top.  The hardware's log2 is off by at most 2^-22 (absolutely, or
-// relatively to a result above one), as much as the hardware's 2^x in the sum itself.
-__device__ __forceinline__ float lse_of(float top, float sum) { return (top + __log2f(sum)) * kLn2; }
+// Natural logarithm of sum * exp(scale * top) / 2^bias.  The hardware's log2 is off by at most 2^-22
+// (absolutely, or relatively to a result above one), as much as the hardware's 2^x in the sum itself.
+__device__ __forceinline__ float lse_of(const DecodeParams& p, float top, float sum) {
+    return fmaf(top, p.scale, (__log2f(sum) - p.bias) * kLn2);
+}
 
 // First and last token of request b, clamped to the page table's capacity.
 __device__ __forceinline__ void range_of(const DecodeParams& p, int b, int64_t* first, int64_t* last) {
@@ -274,9 +279,11 @@ struct Left {
 
 constexpr int kJoinRows = 2;
 
-// What a part weighs whose maximum lies `down` below the largest one (exponents of two).  Never
-// zero: an infinity of V in a part stays one, however little the part weighs.
-__device__ __forceinline__ float part_weight(float down) { return fmaxf(sm100::ex2(down), FLT_MIN); }
+// What a part of maximum `top` weighs where `most` is the largest.  Never zero: an infinity of V in
+// a part stays one, however little the part weighs.
+__device__ __forceinline__ float part_weight(const DecodeParams& p, float top, float most) {
+    return fmaxf(sm100::ex2((top - (most == -INFINITY ? 0.f : most)) * (p.scale * kLog2e)), FLT_MIN);
+}
 
 __device__ __forceinline__ float4 lds_float4(uint32_t at, bool on) {
     float4 v;
@@ -339,13 +346,13 @@ __device__ __forceinline__ void join_parts(const DecodeParams& p, const Runs& r,
             float top = t, sum = mine ? own.sum(own_row) : 0.f;
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float weight = mine ? part_weight(t - (top == -INFINITY ? 0.f : top)) : 0.f;
+            const float weight = mine ? part_weight(p, t, top) : 0.f;
             if (mine) sum *= weight;
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (v == 0 && lane < 8 * R && own_row < ng) {
                 if (!whole) { to.top(own_row) = top; to.sum(own_row) = sum; }
-                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + own_row] = lse_of(top, sum);
+                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq0 + own_row] = lse_of(p, top, sum);
             }
             const float inverse = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
             const uint32_t from = sm100::smem_u32(Part{parts, HG, p.D}.acc(row0));
@@ -450,10 +457,10 @@ struct Walk {
 // Rounding P to 16 bits alone would add an error as large as the output's own rounding, so P
 // goes in as hi + lo, both 16-bit (with 16 heads, where products cost most, 19.7 us instead of
 // 19.1 for 16 requests of up to 16384 tokens).  The base of the power is a maximum seen so far that is
-// only renewed when a logit exceeds it by more than 2^kSlack, which saves the reduction over
-// lanes on most tiles; weights are then at most 2^kSlack instead of 1.  In fp16 they are scaled
-// by 2^kBias besides, so that small ones stay in fp16's normal range; that scale is part of the
-// base and cancels.
+// only renewed when a logit exceeds it by more than kSlack (in exponents of two), which saves the
+// reduction over lanes on most tiles; weights are then at most 2^kSlack instead of 1.  In fp16 they
+// are scaled by 2^kBias besides, so that small ones stay in fp16's normal range; that scale is taken
+// out of the log-sum-exp and cancels in the output.
 // Rows outside the request's range are filled with zeros without being read: what the pool
 // holds there (NaN included) never enters a product.
 // Bound by memory: 8 requests of 32768 tokens (8 x 128, bf16) take 181 us, 5.9 TB/s of K and V,
@@ -495,6 +502,7 @@ struct TcShape {
 };
 
 constexpr float kSlack = 8.f;
+constexpr float tc_bias(bool bf16) { return bf16 ? 0.f : 6.f; }
 
 // Sums of the infinite and NaN elements of V over the tokens [t0, t1) of a request, for dims
 // 8 i + lane / 4 (zero where a column has none): what such a column of the output is, whatever the
@@ -540,7 +548,7 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
     constexpr int kCopies = 16 * kChunks / 32;  // copies per lane for 16 rows of K, and of V
     static_assert(STAGES * Shape::kStage / 2 >= Part::floats(MH, DP) * 4 && STAGES * Shape::kStage % 32 == 0,
                   "two parts fit the warp's ring");
-    constexpr float kBias = kBf16 ? 0.f : 6.f;
+    constexpr float kBias = tc_bias(kBf16);
     sm100::grid_launch_dependents();
     sm100::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -652,8 +660,8 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) issue(s);
 
-        // column x of head block n: base of the power, the logit (unscaled) that renews it
-        // (-inf: none seen), and this lane's share of the sum
+        // column x of head block n: the logit (unscaled, as they all are) that is the base, the one
+        // that renews it (-inf: none seen), and this lane's share of the sum
         float o[DP / 16][NH][4], base[NH][2], limit[NH][2], l[NH][2];
         auto reset = [&]() {
 #pragma unroll
@@ -741,9 +749,9 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
                         const bool renew = v > limit[n][x];
-                        const float b = v * scale2 - kBias;
-                        const float alpha = !renew ? 1.f : limit[n][x] == -INFINITY ? 0.f : sm100::ex2(base[n][x] - b);
-                        base[n][x] = renew ? b : base[n][x];
+                        const float alpha =
+                            !renew ? 1.f : limit[n][x] == -INFINITY ? 0.f : sm100::ex2((base[n][x] - v) * scale2);
+                        base[n][x] = renew ? v : base[n][x];
                         limit[n][x] = renew ? v + slack : limit[n][x];
                         l[n][x] *= alpha;
 #pragma unroll
@@ -761,8 +769,8 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
                 for (int n = 0; n < NH; ++n) {
 #pragma unroll
                     for (int z = 0; z < 2; ++z) {   // tokens g, g + 8
-                        const float w0 = sm100::ex2(fmaf(s[y][n][2 * z], scale2, -base[n][0]));
-                        const float w1 = sm100::ex2(fmaf(s[y][n][2 * z + 1], scale2, -base[n][1]));
+                        const float w0 = sm100::ex2(fmaf(s[y][n][2 * z] - base[n][0], scale2, kBias));
+                        const float w1 = sm100::ex2(fmaf(s[y][n][2 * z + 1] - base[n][1], scale2, kBias));
                         l[n][0] += w0;
                         l[n][1] += w1;
                         const uint32_t h = pack16<kBf16>(w0, w1);
@@ -845,7 +853,7 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
                         const float b = limit[n][x] == -INFINITY ? -INFINITY : base[n][x];
                         if (g == 0 && row < ng) {
                             if (!whole) { part.top(row) = b; part.sum(row) = sum; }
-                            else if (p.lse) p.lse[(int64_t)get.b * p.Hq + h * G + g0 + row] = lse_of(b, sum);
+                            else if (p.lse) p.lse[(int64_t)get.b * p.Hq + h * G + g0 + row] = lse_of(p, b, sum);
                         }
                         if (whole) {
                             const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
@@ -1081,9 +1089,8 @@ decode_f32_kernel(DecodeParams p, int groups, Whole upto) {
 #pragma unroll
                     for (int x = 16; x >= kLpt; x >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
                     const bool renew = v > limit[g];
-                    const float b = v * scale2;
-                    const float alpha = !renew ? 1.f : limit[g] == -INFINITY ? 0.f : sm100::ex2(base[g] - b);
-                    base[g] = renew ? b : base[g];
+                    const float alpha = !renew ? 1.f : limit[g] == -INFINITY ? 0.f : sm100::ex2((base[g] - v) * scale2);
+                    base[g] = renew ? v : base[g];
                     limit[g] = renew ? v + slack : limit[g];
                     l[g] *= alpha;
 #pragma unroll
@@ -1092,7 +1099,7 @@ decode_f32_kernel(DecodeParams p, int groups, Whole upto) {
             }
 #pragma unroll
             for (int g = 0; g < HG; ++g) {
-                s[g] = sm100::ex2(fmaf(s[g], scale2, -base[g]));
+                s[g] = sm100::ex2((s[g] - base[g]) * scale2);
                 l[g] += s[g];
             }
             if (share == 0) {
@@ -1157,7 +1164,7 @@ decode_f32_kernel(DecodeParams p, int groups, Whole upto) {
                     const float b = limit[g] == -INFINITY ? -INFINITY : base[g];
                     if (lane == 0) {
                         if (!whole) { part.top(g) = b; part.sum(g) = sum; }
-                        else if (p.lse) p.lse[(int64_t)get.b * p.Hq + hq] = lse_of(b, sum);
+                        else if (p.lse) p.lse[(int64_t)get.b * p.Hq + hq] = lse_of(p, b, sum);
                     }
                     const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
                     float* to = whole ? static_cast<float*>(p.out) + (int64_t)get.b * p.o_stride_b + (int64_t)hq * p.o_stride_h
@@ -1250,10 +1257,9 @@ decode_any_kernel(DecodeParams p, int groups, Whole upto) {
                 for (int i = 0; i < 8; ++i) s = fmaf(q[g][i], kr[i], s);
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                s *= scale2;
                 const float mn = fmaxf(m[g], s);
                 const float base = mn == -INFINITY ? 0.f : mn;
-                const float alpha = sm100::ex2(m[g] - base), w = sm100::ex2(s - base);
+                const float alpha = sm100::ex2((m[g] - base) * scale2), w = sm100::ex2((s - base) * scale2);
                 m[g] = mn;
                 l[g] = l[g] * alpha + w;
 #pragma unroll
@@ -1289,7 +1295,7 @@ decode_any_kernel(DecodeParams p, int groups, Whole upto) {
             }
             if (lane == 0) {
                 if (!whole) { part.top(g) = m[g]; part.sum(g) = l[g]; }
-                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq] = lse_of(m[g], l[g]);
+                else if (p.lse) p.lse[(int64_t)b * p.Hq + hq] = lse_of(p, m[g], l[g]);
             }
         }
         tile0 = 0;
@@ -1360,7 +1366,7 @@ merge_kernel(DecodeParams p, int groups, int HG) {
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const float weight = part_weight(ml[k].x - (top == -INFINITY ? 0.f : top));
+        const float weight = part_weight(p, ml[k].x, top);
         s_weight[tid + k * kMergeThreads] = weight;
         if (tid + k * kMergeThreads < n) sum += ml[k].y * weight;
     }
@@ -1401,7 +1407,7 @@ merge_kernel(DecodeParams p, int groups, int HG) {
         store_elt(p.out, (int64_t)open.x * p.o_stride_b + (int64_t)hq * p.o_stride_h + d, p.dtype,
                   sum == 0.f ? 0.f : o / sum);
     }
-    if (p.lse && tid == 0) p.lse[(int64_t)open.x * p.Hq + hq] = lse_of(top, sum);
+    if (p.lse && tid == 0) p.lse[(int64_t)open.x * p.Hq + hq] = lse_of(p, top, sum);
 }
 
 namespace {
@@ -1420,7 +1426,7 @@ bool tc_ok(const DecodeParams& p) {
 // A decode kernel and its merge (where there can be something to join), each launched so that its start overlaps the end of the kernel
 // before it (both wait for that kernel's results first).
 template <void (*kernel)(DecodeParams, int, Whole)>
-cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, int TT, cudaStream_t st) {
+cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, int TT, float bias, cudaStream_t st) {
     const int groups = (p.Hq / p.Hkv + HG - 1) / HG;
     // the kernel's shared memory is set once per device (a setting of the function, not of a call)
     static std::atomic<uint64_t> set{0};
@@ -1443,6 +1449,7 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, in
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     DecodeParams q = p;
+    q.bias = bias;
     // (units beyond the tiles of the table's capacity: one for a range that starts within a tile, one
     // or two for the segment itself; doubled, for the search that moves boundaries)
     q.narrow = (double)p.B * p.Hkv * groups * ((double)p.W * p.P / TT + 4) * 2 < 2147483647.0;
@@ -1454,7 +1461,7 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, in
     cfg.gridDim = dim3(kCtas, HG);
     cfg.blockDim = dim3(kMergeWarps * 32);
     cfg.dynamicSmemBytes = 0;
-    return counted(cudaLaunchKernelEx(&cfg, merge_kernel, p, groups, HG), 1);
+    return counted(cudaLaunchKernelEx(&cfg, merge_kernel, q, groups, HG), 1);
 }
 
 template <bool kBf16, int DP, int NH, bool kWhole>
@@ -1468,7 +1475,7 @@ cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
     constexpr int TT = DP <= 128 && !kWide ? 32 : 16, NW = DP <= 64 || kWide ? 8 : 4, STAGES = 2;
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 4096, "shared memory");
-    return launch_pair<decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>>(NW * 32, Shape::kSmem, p, NH * 8, TT, st);
+    return launch_pair<decode_tc_kernel<kBf16, DP, NH, TT, NW, STAGES, kWhole>>(NW * 32, Shape::kSmem, p, NH * 8, TT, tc_bias(kBf16), st);
 }
 
 template <int DP, int NH>
@@ -1501,7 +1508,7 @@ cudaError_t launch_f32(const DecodeParams& p, cudaStream_t st) {
     constexpr int TT = DP <= 64 || kWide ? 16 : 8, NW = DP <= 128 && !kWide ? 8 : 4, STAGES = 2;
     using Shape = F32Shape<DP, HG, TT, NW, STAGES>;
     static_assert(NW <= kMostWarps && Shape::kSmem <= 232448 - 8192, "shared memory");
-    return launch_pair<decode_f32_kernel<DP, HG, TT, NW, STAGES>>(NW * 32, Shape::kSmem, p, HG, TT, st);
+    return launch_pair<decode_f32_kernel<DP, HG, TT, NW, STAGES>>(NW * 32, Shape::kSmem, p, HG, TT, 0.f, st);
 }
 
 template <int DP>
@@ -1523,7 +1530,7 @@ cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
         return launch_f32_heads<256>(p, st);
     }
     if (!tc_ok(p)) return launch_pair<decode_any_kernel>(kAnyWarps * 32,
-                                       kAnyWarps * 2 * Part::floats(kAnyHeads, kMaxHeadDim) * 4, p, kAnyHeads, kAnyTile, st);
+                                       kAnyWarps * 2 * Part::floats(kAnyHeads, kMaxHeadDim) * 4, p, kAnyHeads, kAnyTile, 0.f, st);
     if (p.D <= 64) return launch_tc_heads<64>(p, st);
     if (p.D <= 128) return launch_tc_heads<128>(p, st);
     return launch_tc_heads<256>(p, st);

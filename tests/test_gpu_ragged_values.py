@@ -1,5 +1,5 @@
 """Ragged decode attention on values at the ends of what its types hold (GPU): infinities and
-NaN in tokens that are attended."""
+NaN in tokens that are attended, and logits far beyond the exponents of their weights."""
 
 import math
 
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import razorkv_b200 as R
-from tests.test_gpu_ragged import _pool_case
+from tests.test_gpu_ragged import HALF, U, _pool_case
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,36 @@ def test_infinite_value_in_a_part_of_little_weight(dtype):
     assert bool((out[..., 9] == math.inf).all())
     out[..., 9] = 0
     assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Hq,Hkv,D,lengths", [(8, 2, 64, [500, 1, 37]), (32, 8, 128, [400, 3]), (16, 1, 128, [300, 5]),
+                                              (8, 2, 256, [200, 9]), (6, 2, 17, [333, 2]), (4, 1, 128, [20011])])
+@pytest.mark.parametrize("scale,sign", [(1.0, 1), (0.037, 1), (1.37, -1)])
+def test_logits_beyond_their_weights(dtype, Hq, Hkv, D, lengths, scale, sign):
+    """Scaled logits of 2.7e7 to 1e9.  One product makes a logit, of two numbers of 7 bits, so that
+    it is exact in fp32; every third token has the largest and the others lie 5e5 below and more, so
+    exact weights are 1 and 0, and sums of ones below 2^24 are exact too.  What is left:
+      lse = scale * top + log(count): one rounding of |lse|, one of the logarithm's factor, and the
+        hardware's log2 (2^-22): 2 u |lse| + 2^-20;
+      out = sum of V / count: N sums of 2 u A each, the division, and the output's rounding."""
+    q, kp, vp, table, n, _ = _pool_case(lengths, Hq, Hkv, D, 16, dtype, seed=D)
+    q.zero_()
+    q[..., 0] = 99 * 256.0 * sign
+    top, low = (113, 111) if sign > 0 else (111, 113)
+    for b, m in enumerate(lengths):
+        t = torch.arange(m, device="cuda")
+        k = torch.where(t % 3 == (m - 1) % 3, top * 256.0, low * 256.0)
+        kp[table[b, t // 16], :, t % 16] = 0
+        kp[table[b, t // 16], :, t % 16, 0] = k[:, None].expand(-1, Hkv).to(dtype)
+    got, lse = R.ragged_decode_attention(q, kp, vp, table, n, scale=scale, return_lse=True)
+    s = float(torch.tensor(scale, dtype=torch.float32)) * sign * 99 * 256 * top * 256
+    for b, m in enumerate(lengths):
+        t = torch.arange((m - 1) % 3, m, 3, device="cuda")
+        exact = s + math.log(len(t))
+        assert bool(((lse[b].double() - exact).abs() <= 2 * U * abs(exact) + 2.0 ** -20).all())
+        v = vp[table[b, t // 16], :, t % 16].double()
+        out = v.mean(0).repeat_interleave(Hq // Hkv, 0)
+        A = v.abs().mean(0).repeat_interleave(Hq // Hkv, 0)
+        tol = (2 * len(t) * U + 2.0 ** -20) * A + HALF[dtype] * out.abs() + 2.0 ** -25
+        assert bool(((got[b, :, 0].double() - out).abs() <= tol).all())
