@@ -464,8 +464,9 @@ int rkv_reindex_batch(const rkv_kv_layout* src, const rkv_salience* src_sal,
  *   positions[i]     its position in its request, 0 past the last one
  * The call is granted as a whole or refused as a whole, with error 4 in the error word:
  * pages missing, more than max_new_tokens new tokens, a length outside [0, pt_width * P], more
- * pages given back than the ring holds, or a state that is none.  Refused, out_lengths are
- * lengths, out_state is state, and every slot is -1.  out_lengths may be lengths or
+ * pages given back than the ring has room for beside its free ones, or a state that is none.
+ * Refused, out_lengths are lengths, out_state is state, and every slot is -1.  Every page belongs
+ * to one row: of rows that share pages (the attention takes such tables) each would give them back.  out_lengths may be lengths or
  * new_lengths, and out_state may be state; page_table and ring are updated in place, in
  * entries that lengths and state do not cover, so a repeated call gives the same results. */
 int rkv_ragged_page_tables(const int64_t* lengths, const int64_t* new_lengths, int64_t requests,

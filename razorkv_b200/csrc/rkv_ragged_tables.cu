@@ -20,8 +20,9 @@ static __device__ int g_error;
 // and a, g, s their exclusive prefix sums over r, page j of request r comes from
 // ring[(head + a_r + j - pages(n)) mod C] and page j given back goes to
 // ring[(head + count + g_r + j - pages(m)) mod C].  Pages are taken from the ring's head and
-// given back behind its tail, so what is read and what is written never overlap and no order
-// between CTAs is needed; a stack would hand out the pages that the same call gives back.
+// given back behind its tail, so with count + give <= C, which is checked, what is read and what is
+// written never overlap and no order between CTAs is needed; a stack would hand out the pages that
+// the same call gives back.
 //
 // Every CTA sums need, give and new over all requests (16 bytes each, from L2) instead of
 // waiting for another CTA's sums, then fills chunks of kChunk slot-map entries (one thread
@@ -131,7 +132,7 @@ tables_kernel(TableParams p) {
     const Sums base = block_sums(mine, &total, warp_sums);
     // granted as a whole or not at all
     const bool ok = !bad && total.need <= count && total.fresh <= p.M &&
-                    count - total.need + total.give <= p.C;
+                    count + total.give <= p.C;
 
     // slot map, positions and new table entries
     for (int64_t c0 = (int64_t)blockIdx.x * kChunk; c0 < p.M; c0 += (int64_t)gridDim.x * kChunk) {

@@ -74,8 +74,10 @@ def ragged_page_tables(
     entries, so that a captured step can serve any number of new tokens up to that.
 
     The step is granted as a whole or refused as a whole (pages missing, more than
-    ``max_new_tokens`` new tokens, a length outside [0, W * page_size]): refused, the returned
-    lengths are ``lengths``, every slot is -1 and ``check_device_errors`` raises.
+    ``max_new_tokens`` new tokens, a length outside [0, W * page_size], more pages coming back
+    than the ring has room for beside its free ones): refused, the returned lengths are
+    ``lengths``, every slot is -1 and ``check_device_errors`` raises.  Every page must belong to
+    one request here; rows that share pages, which the attention takes, would each give them back.
 
     ``page_table`` and ``free_ring`` are updated in place.  ``lengths`` and ``free_state`` are
     not unless ``inplace`` is set: the returned ones then ARE those tensors, updated.  Two
