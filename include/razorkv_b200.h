@@ -466,7 +466,9 @@ int rkv_reindex_batch(const rkv_kv_layout* src, const rkv_salience* src_sal,
  * pages missing, more than max_new_tokens new tokens, a length outside [0, pt_width * P], more
  * pages given back than the ring has room for beside its free ones, or a state that is none.
  * Refused, out_lengths are lengths, out_state is state, and every slot is -1.  Every page belongs
- * to one row: of rows that share pages (the attention takes such tables) each would give them back.  out_lengths may be lengths or
+ * to one row: of rows that share pages (the attention takes such tables) each would give them back.
+ * A page id outside the pool is error 2, whether it holds a new token (which gets slot -1), is
+ * taken from the ring, or comes back to it (where it stays).  out_lengths may be lengths or
  * new_lengths, and out_state may be state; page_table and ring are updated in place, in
  * entries that lengths and state do not cover, so a repeated call gives the same results. */
 int rkv_ragged_page_tables(const int64_t* lengths, const int64_t* new_lengths, int64_t requests,

@@ -198,8 +198,9 @@ tables_kernel(TableParams p) {
             const int at = block_running_max(mark[tid], warp_max);
             const int64_t i = c0 + tid;
             if (i >= total.give) continue;
-            p.ring[wrap(head + count + i, p.C)] =
-                p.table[mark_req[at] * p.table_stride + mark_pages[at] + (i - mark_at[at])];
+            const int64_t page = p.table[mark_req[at] * p.table_stride + mark_pages[at] + (i - mark_at[at])];
+            if (page < 0 || page >= p.C) atomicMax(&g_error, kErrPage);
+            p.ring[wrap(head + count + i, p.C)] = page;
         }
     }
 

@@ -59,3 +59,14 @@ def test_requests_that_share_pages_and_both_leave():
     t = R.ragged_page_tables(ints(12, 12), ints(0, 0), table, ring, t.free_state, 4, 0)
     refused(4)
     assert t.lengths.tolist() == [12, 12] and t.free_state.tolist() == [3, 3, 0]
+
+
+def test_a_page_outside_the_pool_comes_back():
+    """It is reported by the call that gives it back, not only by the one that takes it again."""
+    check_device_errors()
+    ring, table = torch.arange(6, device="cuda"), ints(2, 6, 3, -1).reshape(2, 2)
+    t = R.ragged_page_tables(ints(8, 4), ints(4, 4), table, ring, ints(0, 2, 0), 4, 0)
+    refused(2)
+    assert t.lengths.tolist() == [4, 4] and t.free_state.tolist() == [0, 3, 0]
+    R.ragged_page_tables(ints(4, 4), ints(0, 0), table, ring, t.free_state, 4, 0)
+    check_device_errors()       # (an entry behind a request's pages is not looked at)
