@@ -447,8 +447,8 @@ int rkv_reindex_batch(const rkv_kv_layout* src, const rkv_salience* src_sal,
  *
  * What a launch finds wrong on the device (a page id outside the pool, a length outside the
  * table, a step that cannot be granted) is kept in an error word of the library on that
- * device, not in a workspace: rkv_ragged_error reads it.  These calls need no zeroed memory,
- * and calls whose buffers are their own may run at the same time. */
+ * device, not in a workspace: rkv_ragged_error reads it.  Calls whose buffers are their own may
+ * run at the same time. */
 
 /* Page tables and slot map of a step.  Request r holds lengths[r] tokens and is to hold
  * new_lengths[r].  A request that grows takes pages for the tokens its pages do not hold yet
@@ -492,7 +492,9 @@ int rkv_ragged_append(const rkv_kv_layout* pool, const void* k_new, const void* 
  * makes its column infinite, or NaN where both signs meet.  pool->batch is the number of
  * requests and pool->num_tokens the table's capacity, pt_width * P.  scale == 0 selects
  * 1/sqrt(D).  q, pool and out share a dtype; q_len is 1.  A length outside [0, capacity] is
- * read as the nearer bound with error 3, a page id outside the pool as page 0 with error 2. */
+ * read as the nearer bound with error 3, a page id outside the pool as page 0 with error 2.
+ * The workspace's header stays as it is, so other calls may use the same workspace in turn, and
+ * nothing in a workspace that only these calls use needs to be zero. */
 size_t rkv_ragged_decode_attention_workspace_size(const rkv_query* q, const rkv_kv_layout* pool);
 int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
                                 const int64_t* lengths, const int64_t* starts, float scale,

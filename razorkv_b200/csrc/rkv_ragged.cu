@@ -74,7 +74,8 @@ size_t rkv_ragged_decode_attention_workspace_size(const rkv_query* q, const rkv_
     if (!q || !pool || pool->num_kv_heads < 1 || pool->batch < 0 || pool->head_dim < 1 ||
         pool->head_dim > kMaxHeadDim || q->num_heads < 1 || q->num_heads % pool->num_kv_heads)
         return 0;
-    return ragged::decode_workspace_bytes(q->num_heads, pool->num_kv_heads, pool->head_dim);
+    return RKV_WORKSPACE_HEADER_BYTES +
+           ragged::decode_workspace_bytes(q->num_heads, pool->num_kv_heads, pool->head_dim);
 }
 
 int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
@@ -106,7 +107,8 @@ int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
     p.D = pool->head_dim; p.dtype = pool->dtype;
     p.scale = scale > 0.f ? scale : (float)(1.0 / sqrt((double)pool->head_dim));
     p.out = out->out; p.o_stride_b = out->stride_b; p.o_stride_h = out->stride_h; p.lse = lse;
-    p.ws = workspace;
+    // (the header is not used, and left as it is: other calls may share the workspace)
+    p.ws = static_cast<char*>(workspace) + RKV_WORKSPACE_HEADER_BYTES;
     if (p.P < (1ll << 31)) p.div_p = ragged::FastDiv((uint32_t)p.P);
     return status_of(ragged::launch_decode(p, S(stream)));
 }

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import razorkv_b200 as R
+from razorkv_b200 import _lib
 from razorkv_b200._lib import DeviceError
 from razorkv_b200.kernels import check_device_errors
 
@@ -70,3 +71,43 @@ def test_a_page_outside_the_pool_comes_back():
     assert t.lengths.tolist() == [4, 4] and t.free_state.tolist() == [0, 3, 0]
     R.ragged_page_tables(ints(4, 4), ints(0, 0), table, ring, t.free_state, 4, 0)
     check_device_errors()       # (an entry behind a request's pages is not looked at)
+
+
+def test_one_workspace_for_dense_and_ragged_calls():
+    """Every call of the library keeps to a workspace's header: zero at first, and zero after it."""
+    lib = _lib.load()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    B, Hq, Hkv, P, W, D = 2, 8, 2, 16, 40, 128
+    kp, vp = (torch.randn(B * W, Hkv, P, D, generator=g, device="cuda").bfloat16() for _ in "kv")
+    q = torch.randn(B, Hq, 1, D, generator=g, device="cuda").bfloat16()
+    table, n = torch.arange(B * W, device="cuda").reshape(B, W), ints(W * P, 77)
+    want = R.ragged_decode_attention(q, kp, vp, table, n)
+    # the same rows as a dense cache [B, Hkv, T, D]
+    k, v = (t.reshape(B, W, Hkv, P, D).transpose(1, 2).reshape(B, Hkv, W * P, D).contiguous() for t in (kp, vp))
+    dense = _lib.KVLayout(k=k.data_ptr(), v=v.data_ptr(), dtype=_lib.dtype_code(q.dtype), head_dim=D, batch=B,
+                          num_kv_heads=Hkv, stride_b=Hkv * W * P * D, stride_h=W * P * D, stride_t=D,
+                          num_tokens=W * P)
+    pool = _lib.KVLayout(k=kp.data_ptr(), v=vp.data_ptr(), dtype=_lib.dtype_code(q.dtype), head_dim=D, batch=B,
+                         num_kv_heads=Hkv, stride_h=P * D, stride_p=Hkv * P * D, stride_t=D, page_size=P,
+                         num_slots=B * W, page_table=table.data_ptr(), pt_stride_b=W, num_tokens=W * P)
+    out, again = torch.empty_like(q), torch.empty_like(q)
+    qs = _lib.Query(q.data_ptr(), _lib.dtype_code(q.dtype), Hq, 1, Hq * D, D, D)
+    size = max(lib.rkv_decode_attention_workspace_size(qs, dense),
+               lib.rkv_ragged_decode_attention_workspace_size(qs, pool))
+    ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    first = None
+    for _ in range(3):
+        o = _lib.Output(out.data_ptr(), _lib.dtype_code(q.dtype), 0, Hq * D, D, D)
+        assert lib.rkv_ragged_decode_attention(qs, pool, n.data_ptr(), None, 0.0, o, None, ws.data_ptr(), size,
+                                               stream) == 0
+        assert torch.equal(out, want)
+        assert int(ws[:65536].count_nonzero()) == 0
+        o = _lib.Output(again.data_ptr(), _lib.dtype_code(q.dtype), 0, Hq * D, D, D)
+        assert lib.rkv_decode_attention(qs, dense, 0.0, 0, o, ws.data_ptr(), size, stream) == 0
+        assert int(ws[:65536].count_nonzero()) == 0
+        first = again.clone() if first is None else first
+        assert torch.equal(again, first)
+    # request 0 has all its tokens in both
+    assert torch.allclose(first[0].float(), want[0].float(), atol=2e-2, rtol=1e-2)
+    check_device_errors()
