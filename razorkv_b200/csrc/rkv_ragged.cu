@@ -95,6 +95,7 @@ int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
     if (pool->batch * q->num_heads > 0x7fffffff) return RKV_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < rkv_ragged_decode_attention_workspace_size(q, pool))
         return RKV_ERR_WORKSPACE_TOO_SMALL;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return RKV_ERR_ALIGNMENT;
     ragged::DecodeParams p{};
     p.q = q->q; p.q_stride_b = q->stride_b; p.q_stride_h = q->stride_h;
     p.k = pool->k; p.v = pool->v;
