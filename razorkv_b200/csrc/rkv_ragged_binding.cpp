@@ -263,15 +263,16 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-// Lengths and used table entries, read back.
-void validate(const at::Tensor& table, const at::Tensor& lengths, const rkv_kv_layout& lay) {
+// Lengths, and the table entries of tokens that are attended, read back.
+void validate(const at::Tensor& table, const at::Tensor& lengths, const at::Tensor* starts, const rkv_kv_layout& lay) {
     const int64_t lo = lengths.min().item<int64_t>(), hi = lengths.max().item<int64_t>();
     if (lo < 0 || hi > lay.num_tokens)
         refuse(PyExc_IndexError, "lengths must lie in [0, " + std::to_string(lay.num_tokens) + "], got [" +
                                      std::to_string(lo) + ", " + std::to_string(hi) + "]");
     if (!table.numel()) return;
-    const at::Tensor used = (at::arange(table.size(1), table.options()) * lay.page_size).unsqueeze(0) <
-                            lengths.unsqueeze(1);
+    const at::Tensor first = (at::arange(table.size(1), table.options()) * lay.page_size).unsqueeze(0);
+    at::Tensor used = first < lengths.unsqueeze(1);
+    if (starts) used = used & (first + lay.page_size > starts->unsqueeze(1)) & (*starts < lengths).unsqueeze(1);
     if ((used & ((table < 0) | (table >= lay.num_slots))).any().item<bool>())
         refuse(PyExc_IndexError, "page_table entries must lie in [0, " + std::to_string(lay.num_slots) + ")");
 }
@@ -322,7 +323,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         }
         if (want_checks) {      // (on any device)
             lay.num_tokens = pages.size(1) * lay.page_size;
-            if (B) validate(pages, lengths, lay);
+            if (B) validate(pages, lengths, starts, lay);
         }
         const auto index = device_of(query, &kp, &vp, &pages, &lengths, starts, given);
         const Launch launch(index);

@@ -16,3 +16,24 @@ def test_workspace_alignment():
     size = lib.rkv_ragged_decode_attention_workspace_size(q, pool)
     for at in (8, 24, 1):
         assert lib.rkv_ragged_decode_attention(q, pool, 16, None, 0.0, o, None, at, size, None) == 5
+
+
+def _attend(lengths, starts, table, **changes):
+    """A call that ends at the device (its tensors are on the CPU), unless its values are refused."""
+    return R.ragged_decode_attention(
+        torch.zeros(len(lengths), 4, 1, 8), torch.zeros(5, 2, 4, 8), torch.zeros(5, 2, 4, 8),
+        torch.tensor(table), torch.tensor(lengths), starts=torch.tensor(starts), validate=True, **changes)
+
+
+def test_validation_looks_at_the_pages_of_the_window():
+    # pages in front of the window were given back; requests without a token in their window use none
+    for lengths, starts, table in (([12, 5], [4, 0], [[-1, 1, 2], [3, 4, 9]]),
+                                   ([12, 5], [8, 4], [[-1, -1, 2], [9, 4, 9]]),
+                                   ([12, 5], [11, 5], [[9, 9, 0], [9, 9, 9]]),
+                                   ([12, 5], [1 << 40, 7], [[9, 9, 9], [9, 9, 9]])):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            _attend(lengths, starts, table)
+    for starts, table in (([3, 0], [[-1, 1, 2], [3, 4, 9]]), ([4, 0], [[-1, 1, 5], [3, 4, 9]]),
+                          ([4, 4], [[-1, 1, 2], [3, 9, 9]])):
+        with pytest.raises(IndexError, match="page_table"):
+            _attend([12, 5], starts, table)
