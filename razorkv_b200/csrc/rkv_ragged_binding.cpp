@@ -269,6 +269,8 @@ void validate(const at::Tensor& table, const at::Tensor& lengths, const at::Tens
     if (lo < 0 || hi > lay.num_tokens)
         refuse(PyExc_IndexError, "lengths must lie in [0, " + std::to_string(lay.num_tokens) + "], got [" +
                                      std::to_string(lo) + ", " + std::to_string(hi) + "]");
+    if (starts && starts->min().item<int64_t>() < 0)
+        refuse(PyExc_IndexError, "starts must not be negative, got " + std::to_string(starts->min().item<int64_t>()));
     if (!table.numel()) return;
     const at::Tensor first = (at::arange(table.size(1), table.options()) * lay.page_size).unsqueeze(0);
     at::Tensor used = first < lengths.unsqueeze(1);

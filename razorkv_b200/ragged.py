@@ -125,8 +125,9 @@ def ragged_decode_attention(
     way into the output (an infinite element of V makes its column infinite, or NaN where both
     signs meet).  ``scale`` defaults to 1 / sqrt(D).
 
-    Lengths outside [0, W * P] and page ids outside the pool are kept inside them and raised by
-    ``check_device_errors``; ``validate`` checks them on the host first (one device sync)."""
+    Lengths outside [0, W * P], negative starts and page ids of attended tokens outside the pool
+    are kept inside and raised by ``check_device_errors``; ``validate`` checks them on the host
+    first (a few device syncs)."""
     return _lib.ragged().decode(query, key_pool, value_pool, page_table, lengths, scale, starts,
                                 return_lse, out, validate)
 

@@ -37,3 +37,10 @@ def test_validation_looks_at_the_pages_of_the_window():
                           ([4, 4], [[-1, 1, 2], [3, 9, 9]])):
         with pytest.raises(IndexError, match="page_table"):
             _attend([12, 5], starts, table)
+
+
+def test_validation_refuses_negative_starts():
+    with pytest.raises(IndexError, match="starts"):
+        _attend([12, 5], [4, -1], [[0, 1, 2], [3, 4, 0]])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        _attend([12, 5], [4, 0], [[0, 1, 2], [3, 4, 0]])
