@@ -4,7 +4,8 @@
  * Every entry point takes plain device pointers, element strides and sizes, enqueues its
  * work on the given CUDA stream (passed as void*, a cudaStream_t; NULL = legacy default
  * stream) and returns an rkv_status.  Nothing here allocates, frees or synchronises
- * (rkv_ragged_error, which reads an error word back, waits for the device): the
+ * (rkv_ragged_error, which reads an error word back, waits for the device, and
+ * rkv_ragged_stream_error for its stream): the
  * caller owns every buffer, including the workspaces whose sizes the *_workspace_size
  * queries report, and all sizes needed for a launch are host-known.  Calls are
  * stream-ordered; the library keeps no per-call state, so calls from several host threads
@@ -502,8 +503,11 @@ int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
                                 size_t workspace_bytes, void* stream);
 
 /* Waits for the current device, reads the ragged calls' error word there (0: none; the largest
- * code otherwise) and, with clear != 0, resets it. */
+ * code otherwise) and, with clear != 0, resets it.  The word is one for all streams of the device:
+ * of several callers, the first to ask is told.  rkv_ragged_stream_error waits for the stream
+ * alone, and is sure to see the errors of what was enqueued on it before. */
 int rkv_ragged_error(int clear, int* code);
+int rkv_ragged_stream_error(int clear, int* code, void* stream);
 
 #ifdef __cplusplus
 }

@@ -141,6 +141,7 @@ _SIGNATURES = {
     "rkv_ragged_decode_attention": (ctypes.c_int, [P(Query), P(KVLayout), c_vp, c_vp, c_f32,
                                                    P(Output), c_vp, c_vp, c_sz, c_vp]),
     "rkv_ragged_error": (ctypes.c_int, [ctypes.c_int, P(c_i32)]),
+    "rkv_ragged_stream_error": (ctypes.c_int, [ctypes.c_int, P(c_i32), c_vp]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -210,12 +211,13 @@ def ragged_devices():
 
 
 def ragged_error(device_index: int, clear: bool = True) -> int:
-    """The ragged operators' error word of a device (waits for the device)."""
+    """The ragged operators' error word of a device (waits for its current stream)."""
     code = c_i32(0)
     with torch.cuda.device(device_index):
-        check(load().rkv_ragged_error(1 if clear else 0, code), "rkv_ragged_error")
+        check(load().rkv_ragged_stream_error(1 if clear else 0, code,
+                                             torch.cuda.current_stream().cuda_stream),
+              "rkv_ragged_stream_error")
     return code.value
-
 
 
 class DeviceError(RazorKVError):

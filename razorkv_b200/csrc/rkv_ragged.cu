@@ -114,15 +114,22 @@ int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
     return status_of(ragged::launch_decode(p, S(stream)));
 }
 
-int rkv_ragged_error(int clear, int* code) {
+int rkv_ragged_stream_error(int clear, int* code, void* stream) {
     if (!code) return RKV_ERR_INVALID_ARGUMENT;
     *code = 0;
     int a = 0, b = 0;
-    if (cudaDeviceSynchronize() != cudaSuccess || ragged::read_table_error(clear, &a) != cudaSuccess ||
-        ragged::read_decode_error(clear, &b) != cudaSuccess)
+    if (ragged::read_table_error(clear, &a, S(stream)) != cudaSuccess ||
+        ragged::read_decode_error(clear, &b, S(stream)) != cudaSuccess)
         return RKV_ERR_CUDA;
     *code = a > b ? a : b;
     return RKV_OK;
+}
+
+int rkv_ragged_error(int clear, int* code) {
+    if (!code) return RKV_ERR_INVALID_ARGUMENT;
+    *code = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess) return RKV_ERR_CUDA;
+    return rkv_ragged_stream_error(clear, code, nullptr);
 }
 
 }  // extern "C"

@@ -66,9 +66,27 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t st);
 size_t decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D);
 cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st);
 
-// Reads (and with clear resets) the error word of one translation unit on the current device.
-cudaError_t read_table_error(int clear, int* code);
-cudaError_t read_decode_error(int clear, int* code);
+// Reads (and with clear resets) the error word of one translation unit on the current device, in
+// the stream's order, and waits for that.
+cudaError_t read_table_error(int clear, int* code, cudaStream_t st);
+cudaError_t read_decode_error(int clear, int* code, cudaStream_t st);
+
+#ifdef __CUDACC__
+// The above for one word.  It is reset only where it is still the code that was read: a larger one
+// that another stream's kernel has set since is for the next caller.
+static __global__ void clear_error_kernel(int* word, int code) { atomicCAS(word, code, 0); }
+
+inline cudaError_t read_error(const void* symbol, int clear, int* code, cudaStream_t st) {
+    void* word = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&word, symbol);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(code, word, sizeof(int), cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess || !clear || !*code) return e;
+    clear_error_kernel<<<1, 1, 0, st>>>(static_cast<int*>(word), *code);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
+}
+#endif
 
 }  // namespace ragged
 }  // namespace rkv

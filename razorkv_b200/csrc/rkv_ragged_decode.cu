@@ -1536,13 +1536,8 @@ cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
     return launch_tc_heads<256>(p, st);
 }
 
-cudaError_t read_decode_error(int clear, int* code) {
-    cudaError_t e = cudaMemcpyFromSymbol(code, g_error, sizeof(int));
-    if (e == cudaSuccess && clear && *code) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(g_error, &zero, sizeof(int));
-    }
-    return e;
+cudaError_t read_decode_error(int clear, int* code, cudaStream_t st) {
+    return read_error(&g_error, clear, code, st);
 }
 
 }  // namespace ragged

@@ -336,13 +336,8 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t st) {
     return launch(append_kernel<uint32_t>, ctas, kAppendThreads, st, p, dt, dr, per_token, per_row, elts, tokens);
 }
 
-cudaError_t read_table_error(int clear, int* code) {
-    cudaError_t e = cudaMemcpyFromSymbol(code, g_error, sizeof(int));
-    if (e == cudaSuccess && clear && *code) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(g_error, &zero, sizeof(int));
-    }
-    return e;
+cudaError_t read_table_error(int clear, int* code, cudaStream_t st) {
+    return read_error(&g_error, clear, code, st);
 }
 
 }  // namespace ragged

@@ -107,7 +107,8 @@ class Workspace:
 def check_device_errors(device=None) -> None:
     """Raise ``razorkv_b200._lib.DeviceError`` if a decode kernel recorded a device-side
     error on ``device`` (every device when None) since the last check; clears the flags.
-    Synchronises the device: call it at sync points, not per step."""
+    Waits for the device's current stream (launches of other streams may not have recorded
+    theirs yet): call it at sync points, not per step."""
     Workspace.check_errors(device)
 
 

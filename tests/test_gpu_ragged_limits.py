@@ -111,3 +111,20 @@ def test_one_workspace_for_dense_and_ragged_calls():
     # request 0 has all its tokens in both
     assert torch.allclose(first[0].float(), want[0].float(), atol=2e-2, rtol=1e-2)
     check_device_errors()
+
+
+def test_the_check_waits_for_its_own_stream_only():
+    """Work of another stream (half a second of it) goes on while the errors are read."""
+    check_device_errors()
+    R.ragged_append(torch.ones(1, 1, 8, device="cuda"), torch.ones(1, 1, 8, device="cuda"),
+                    torch.zeros(1, 1, 4, 8, device="cuda"), torch.zeros(1, 1, 4, 8, device="cuda"), ints(4))
+    other, done = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(1_000_000_000)
+        done.record()
+    refused(2)
+    check_device_errors()       # read and cleared
+    busy = not done.query()
+    torch.cuda.synchronize()
+    assert busy
