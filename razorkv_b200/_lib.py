@@ -6,12 +6,12 @@ import fails with an error that says how to build it.  There is no CPU fallback.
 
 import ctypes
 import os
+import sys
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "librazorkv_b200.so")
-RAGGED_PATH = os.path.join(_HERE, "_lib", "_ragged.so")
 
 c_i64 = ctypes.c_int64
 c_i32 = ctypes.c_int32
@@ -184,17 +184,22 @@ DEVICE_ERRORS = {
 _ragged = None
 
 
+def ragged_path() -> str:
+    """File of the ragged operators' binding.  It is compiled against torch's and Python's C++
+    interfaces, so their versions are part of its name: each version has its own."""
+    return os.path.join(_HERE, "_lib", f"_ragged.{sys.implementation.cache_tag}-torch-{torch.__version__}.so")
+
+
 def ragged():
-    """The ragged operators' binding (_ragged.so), bound to the library's entries."""
+    """The ragged operators' binding, bound to the library's entries."""
     global _ragged
     if _ragged is None:
-        lib = load()
-        if not os.path.exists(RAGGED_PATH):
-            raise ImportError(f"{RAGGED_PATH} is missing; build it with `python -m razorkv_b200.build`")
+        lib, path = load(), ragged_path()
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing; build it with `python -m razorkv_b200.build`")
         from importlib.machinery import ExtensionFileLoader
         from importlib.util import module_from_spec, spec_from_file_location
-        spec = spec_from_file_location("_ragged", RAGGED_PATH,
-                                       loader=ExtensionFileLoader("_ragged", RAGGED_PATH))
+        spec = spec_from_file_location("_ragged", path, loader=ExtensionFileLoader("_ragged", path))
         module = module_from_spec(spec)
         spec.loader.exec_module(module)
         module.bind(RazorKVError, *(ctypes.cast(getattr(lib, name), c_vp).value for name in (

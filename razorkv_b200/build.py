@@ -1,5 +1,5 @@
-"""Builds librazorkv_b200.so (the C-ABI CUDA library) in-tree for sm_100a, and _ragged.so, the
-ragged operators' binding of it to torch tensors.
+"""Builds librazorkv_b200.so (the C-ABI CUDA library) in-tree for sm_100a, and _ragged.*.so, the
+ragged operators' binding of it to the tensors of the torch that builds it.
 
     python -m razorkv_b200.build            # incremental
     python -m razorkv_b200.build --force    # rebuild every object
@@ -19,7 +19,6 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(HERE, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "librazorkv_b200.so")
-BINDING_PATH = os.path.join(LIB_DIR, "_ragged.so")
 
 SOURCES = ["rkv_capi.cu", "rkv_generic.cu", "rkv_decode_sm100.cu", "rkv_noalloc.cu",
            "rkv_ragged.cu", "rkv_ragged_tables.cu", "rkv_ragged_decode.cu"]
@@ -80,7 +79,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
 def _build_binding(force: bool):
     src = os.path.join(CSRC, "rkv_ragged_binding.cpp")
     header = os.path.join(ROOT, "include", "razorkv_b200.h")
-    if not force and not _stale(BINDING_PATH, [src, header, __file__]):
+    from ._lib import ragged_path
+    path = ragged_path()
+    if not force and not _stale(path, [src, header, __file__]):
         return
     import sysconfig
 
@@ -90,12 +91,12 @@ def _build_binding(force: bool):
     dirs = include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-I{d}" for d in dirs), src, "-o", BINDING_PATH, *(f"-L{d}" for d in library_paths()),
+           *(f"-I{d}" for d in dirs), src, "-o", path, *(f"-L{d}" for d in library_paths()),
            "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("build of _ragged.so failed")
+        raise RuntimeError(f"build of {path} failed")
 
 
 if __name__ == "__main__":

@@ -44,3 +44,13 @@ def test_validation_refuses_negative_starts():
         _attend([12, 5], [4, -1], [[0, 1, 2], [3, 4, 0]])
     with pytest.raises(RuntimeError, match="CUDA"):
         _attend([12, 5], [4, 0], [[0, 1, 2], [3, 4, 0]])
+
+
+def test_the_binding_is_the_one_of_this_torch(monkeypatch):
+    """A binary of another torch version, whose C++ interface may differ, is not loaded."""
+    monkeypatch.setattr(_lib, "_ragged", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0+other")
+    with pytest.raises(ImportError, match="razorkv_b200.build"):
+        _lib.ragged()
+    monkeypatch.undo()
+    assert _lib.ragged().devices() == 0 or torch.cuda.is_available()
