@@ -40,6 +40,8 @@ int rkv_ragged_page_tables(const int64_t* lengths, const int64_t* new_lengths, i
     // page_size * pt_width is a token count, page_size * ring_size a slot id
     if (pt_width > INT64_MAX / page_size || ring_size > INT64_MAX / page_size)
         return RKV_ERR_INVALID_ARGUMENT;
+    // and so is the sum of it over all requests
+    if (requests > 0 && pt_width * page_size > INT64_MAX / requests) return RKV_ERR_INVALID_ARGUMENT;
     if (!ring || !state || !out_state || !token_starts) return RKV_ERR_INVALID_ARGUMENT;
     if (requests > 0 && (!lengths || !new_lengths || !out_lengths)) return RKV_ERR_INVALID_ARGUMENT;
     if (requests > 0 && pt_width > 0 && !page_table) return RKV_ERR_INVALID_ARGUMENT;

@@ -54,3 +54,15 @@ def test_the_binding_is_the_one_of_this_torch(monkeypatch):
         _lib.ragged()
     monkeypatch.undo()
     assert _lib.ragged().devices() == 0 or torch.cuda.is_available()
+
+
+def test_token_counts_beyond_64_bits_are_refused():
+    """The step's sums are 64-bit numbers: all requests' tables together have room for fewer tokens."""
+    lib = _lib.load()
+
+    def call(requests, width, page):
+        return lib.rkv_ragged_page_tables(16, 16, requests, page, 16, width, width, 16, 1, 16, 16, 16, 16, 16, 8,
+                                          16, None)
+
+    for requests, width, page in ((4, 2, 1 << 61), (3, 1, 1 << 62), (1 << 22, 5, 1 << 40)):
+        assert call(requests, width, page) == 1
