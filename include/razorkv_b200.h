@@ -492,7 +492,7 @@ int rkv_ragged_append(const rkv_kv_layout* pool, const void* k_new, const void* 
  * holds outside the tokens (NaN included) has no effect; an infinite element of V in one of them
  * makes its column infinite, or NaN where both signs meet.  pool->batch is the number of
  * requests and pool->num_tokens the table's capacity, pt_width * P.  scale == 0 selects
- * 1/sqrt(D).  q, pool and out share a dtype; q_len is 1.  A length outside [0, capacity], or a
+ * 1/sqrt(D), and scale * log2 e has to be finite.  q, pool and out share a dtype; q_len is 1.  A length outside [0, capacity], or a
  * negative start, is read as the nearer bound with error 3, a page id outside the pool as page 0 with error 2.
  * The workspace starts on a 16-byte boundary (RKV_ERR_ALIGNMENT).  Its header stays as it is, so other calls may use the same workspace in turn, and
  * nothing in a workspace that only these calls use needs to be zero. */

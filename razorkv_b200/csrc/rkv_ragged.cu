@@ -91,7 +91,7 @@ int rkv_ragged_decode_attention(const rkv_query* q, const rkv_kv_layout* pool,
     if (q->num_heads < 1 || q->num_heads % pool->num_kv_heads) return RKV_ERR_INVALID_ARGUMENT;
     if (pool->batch < 0 || pool->num_tokens < 0 || pool->num_tokens % pool->page_size)
         return RKV_ERR_INVALID_ARGUMENT;
-    if (!(scale >= 0.f) || isinf(scale)) return RKV_ERR_INVALID_ARGUMENT;
+    if (!(scale >= 0.f) || isinf(scale * 1.44269504f)) return RKV_ERR_INVALID_ARGUMENT;    // (log2 e)
     if (pool->batch == 0) return RKV_OK;
     if (!lengths || (pool->num_tokens > 0 && !pool->page_table)) return RKV_ERR_INVALID_ARGUMENT;
     if (pool->batch * q->num_heads > 0x7fffffff) return RKV_ERR_UNSUPPORTED;

@@ -314,8 +314,8 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (a[5] != Py_None) {
             scale = PyFloat_AsDouble(a[5]);
             if (scale == -1.0 && PyErr_Occurred()) return nullptr;
-            if (!(scale > 0.0 && std::isfinite((float)scale) && (float)scale > 0.f))
-                refuse(PyExc_ValueError, "scale must be positive and finite, got " + std::to_string(scale));
+            if (!(scale > 0.0 && std::isfinite((float)scale * 1.44269504f) && (float)scale > 0.f))   // (log2 e)
+                refuse(PyExc_ValueError, "scale must be positive and below 2.35e38, got " + std::to_string(scale));
         }
         if (given) {
             if (given->sizes() != query.sizes() || given->scalar_type() != query.scalar_type() ||

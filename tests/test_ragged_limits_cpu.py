@@ -66,3 +66,20 @@ def test_token_counts_beyond_64_bits_are_refused():
 
     for requests, width, page in ((4, 2, 1 << 61), (3, 1, 1 << 62), (1 << 22, 5, 1 << 40)):
         assert call(requests, width, page) == 1
+
+
+def test_scales_whose_exponent_overflows_are_refused():
+    """Weights are powers of two of scale * log2 e, which has to be a number too."""
+    q, pool, table = torch.zeros(2, 4, 1, 8), torch.zeros(5, 2, 4, 8), torch.zeros(2, 3, dtype=torch.int64)
+    call = lambda scale: R.ragged_decode_attention(q, pool, pool, table, torch.tensor([1, 7]), scale)  # noqa: E731
+    for scale in (2.4e38, 3.4e38):
+        with pytest.raises(ValueError, match="scale"):
+            call(scale)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        call(2.3e38)
+    lib = _lib.load()
+    lay = _lib.KVLayout(k=16, v=16, dtype=2, head_dim=128, batch=2, num_kv_heads=2, stride_h=2048,
+                        stride_p=4096, stride_t=128, page_size=16, num_slots=7, page_table=16,
+                        pt_stride_b=3, num_tokens=48)
+    qs, o = _lib.Query(16, 2, 8, 1, 1024, 128, 128), _lib.Output(16, 2, 0, 1024, 128, 128)
+    assert lib.rkv_ragged_decode_attention(qs, lay, 16, None, 3e38, o, None, None, 0, None) == 1
