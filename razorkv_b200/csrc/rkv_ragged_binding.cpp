@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -76,6 +77,12 @@ void want_int64(const at::Tensor& t, int64_t dim, const char* name) {
 void want_written(const at::Tensor& t, const char* name) {
     if (t.numel() && !t.is_contiguous())
         refuse(PyExc_ValueError, std::string(name) + " is updated in place and must be contiguous");
+}
+
+bool on_itself(const at::Tensor& t) { return at::has_internal_overlap(t) == at::MemOverlap::Yes; }
+bool on_another(const at::Tensor& a, const at::Tensor& b) {
+    const auto s = at::get_overlap_status(a, b);
+    return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
 }
 
 int dtype_code(at::ScalarType t) {
@@ -245,6 +252,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (key.scalar_type() != kp.scalar_type() || value.scalar_type() != kp.scalar_type())
             refuse(PyExc_TypeError, std::string("key and value must have the pool's dtype ") +
                                         c10::toString(kp.scalar_type()));
+        if (on_itself(kp) || on_itself(vp) || on_another(kp, vp))
+            refuse(PyExc_ValueError, "the rows of key_pool and value_pool are written and must not overlap");
         const auto index = device_of(key, &value, &kp, &vp, &slots);
         if (T == 0) Py_RETURN_NONE;
         const Launch launch(index);
@@ -322,6 +331,8 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 given->stride(3) != 1)
                 refuse(PyExc_ValueError, "out must have the query's shape and dtype, with contiguous rows");
             if (B && given->data_ptr() == query.data_ptr()) refuse(PyExc_ValueError, "out must not be the query");
+            if (on_itself(*given) || on_another(*given, query) || on_another(*given, kp) || on_another(*given, vp))
+                refuse(PyExc_ValueError, "out's rows must not overlap each other, the query or the pools");
         }
         if (want_checks) {      // (on any device)
             lay.num_tokens = pages.size(1) * lay.page_size;

@@ -83,3 +83,25 @@ def test_scales_whose_exponent_overflows_are_refused():
                         pt_stride_b=3, num_tokens=48)
     qs, o = _lib.Query(16, 2, 8, 1, 1024, 128, 128), _lib.Output(16, 2, 0, 1024, 128, 128)
     assert lib.rkv_ragged_decode_attention(qs, lay, 16, None, 3e38, o, None, None, 0, None) == 1
+
+
+def test_buffers_that_are_written_must_not_overlap():
+    """Rows that lie on one another, or on what the call reads, would be written in any order."""
+    table, n = torch.zeros(2, 3, dtype=torch.int64), torch.tensor([1, 7])
+    pool, q = torch.zeros(5, 2, 4, 8), torch.zeros(2, 4, 1, 8)
+    both = torch.zeros(2 * 4 * 8 + 8)
+    joint = torch.zeros(2, 12, 1, 8)       # queries and outputs in columns of one tensor: apart
+    for query, out, ok in ((q, torch.zeros(1, 4, 1, 8).expand(2, 4, 1, 8), False),
+                           (q, torch.zeros(2, 1, 1, 8).expand(2, 4, 1, 8), False),
+                           (both[:64].view(2, 4, 1, 8), both[8:].view(2, 4, 1, 8), False),
+                           (q, pool.view(-1)[:64].view(2, 4, 1, 8), False),
+                           (joint[:, :4], joint[:, 8:], True)):
+        with pytest.raises(RuntimeError if ok else ValueError, match="CUDA" if ok else "out"):
+            R.ragged_decode_attention(query, pool, pool, table, n, out=out)
+    rows, slots = torch.zeros(3, 2, 8), torch.tensor([0, 5, -1])
+    pair = torch.zeros(5, 2, 2, 4, 8)      # K and V of a page side by side: apart
+    for kp, vp, ok in ((pool, pool, False), (torch.zeros(1, 2, 4, 8).expand(5, 2, 4, 8),
+                                             torch.zeros(1, 2, 4, 8).expand(5, 2, 4, 8), False),
+                       (pair[:, 0], pair[:, 1], True), (pool, torch.zeros_like(pool), True)):
+        with pytest.raises(RuntimeError if ok else ValueError, match="CUDA" if ok else "pool"):
+            R.ragged_append(rows, rows, kp, vp, slots)
