@@ -481,7 +481,7 @@ int rkv_ragged_page_tables(const int64_t* lengths, const int64_t* new_lengths, i
 
 /* Writes row t of k_new / v_new [n_new, Hkv, D] (element strides new_stride_t and
  * new_stride_h) to the pool's slot slot_map[t].  Negative slots are skipped; one past the pool
- * is skipped with error 2.  Two rows of one slot: either may be the one that stays. */
+ * is skipped with error 2.  Two rows of one slot: pieces of both may be left there. */
 int rkv_ragged_append(const rkv_kv_layout* pool, const void* k_new, const void* v_new,
                       int64_t new_stride_t, int64_t new_stride_h, int64_t n_new,
                       const int64_t* slot_map, void* stream);

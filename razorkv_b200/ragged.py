@@ -97,7 +97,7 @@ def ragged_append(
     [num_slots, Hkv, P, D]: row ``slot % P`` of page ``slot // P``.
 
     Negative slots are skipped (a padded tail); one past the pool is skipped and raised by
-    ``check_device_errors``.  Rows of one slot must not repeat: either may be the one left."""
+    ``check_device_errors``.  A slot must not repeat: what is left there may be pieces of both rows."""
     _lib.ragged().append(key, value, key_pool, value_pool, slot_map)
 
 
