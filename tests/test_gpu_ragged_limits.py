@@ -1,5 +1,7 @@
 """Limits of the ragged operators: inconsistent rings, and what calls share (GPU)."""
 
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -7,6 +9,7 @@ import razorkv_b200 as R
 from razorkv_b200 import _lib
 from razorkv_b200._lib import DeviceError
 from razorkv_b200.kernels import check_device_errors
+from tests.test_gpu_ragged import _pool_case
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +131,43 @@ def test_the_check_waits_for_its_own_stream_only():
     busy = not done.query()
     torch.cuda.synchronize()
     assert busy
+
+
+@pytest.mark.parametrize("mode", [torch.inference_mode, torch.no_grad, torch.enable_grad])
+def test_results_are_ordinary_tensors(mode):
+    """The step's five results lie on two allocations: each can be written, viewed and kept alone."""
+    with mode():
+        ring, state = R.ragged_free_ring(8, "cuda")
+        table = torch.zeros(2, 4, dtype=torch.int64, device="cuda")
+        t = R.ragged_page_tables(ints(0, 0), ints(5, 3), table, ring, state, 4, 10)
+        want = [x.clone() for x in t]
+        for i, x in enumerate(t):
+            assert x.is_contiguous() and not x.requires_grad and x.is_inference() == (mode is torch.inference_mode)
+            x.add_(1000 + i)
+            assert all(torch.equal(y, w if j != i else w + 1000 + i) for j, (y, w) in enumerate(zip(t, want)))
+            x.copy_(want[i])
+        kp, vp = torch.zeros(2, 8, 2, 4, 8, device="cuda").unbind(0)
+        rows = torch.ones(10, 2, 8, device="cuda", requires_grad=mode is torch.enable_grad)
+        R.ragged_append(rows, rows, kp, vp, t.slot_map)
+        q = torch.zeros(2, 4, 1, 8, device="cuda", requires_grad=mode is torch.enable_grad)
+        out, lse = R.ragged_decode_attention(q, kp, vp, table, t.lengths, return_lse=True)
+        assert not out.requires_grad and bool((out == 1).all())
+        assert lse.exp().round().tolist() == [[5.0] * 4, [3.0] * 4]
+    check_device_errors()
+
+
+def test_calls_from_several_host_threads():
+    """Threads that never made a CUDA call, each on a stream of its own, all at the same time."""
+    cases = [_pool_case([n, 1, n // 3], 8, 2, 128, 16, torch.bfloat16, seed=n) for n in (300, 2000, 9000, 40)]
+    want = [R.ragged_decode_attention(*c[:5], return_lse=True) for c in cases]
+    torch.cuda.synchronize()
+
+    def work(case):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [R.ragged_decode_attention(*case[:5], return_lse=True) for _ in range(50)]
+            torch.cuda.current_stream().synchronize()
+        return got
+
+    with ThreadPoolExecutor(len(cases)) as pool:
+        for got, (out, lse) in zip(pool.map(work, cases), want):
+            assert all(torch.equal(a, out) and torch.equal(b, lse) for a, b in got)

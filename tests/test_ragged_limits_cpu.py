@@ -105,3 +105,15 @@ def test_buffers_that_are_written_must_not_overlap():
                        (pair[:, 0], pair[:, 1], True), (pool, torch.zeros_like(pool), True)):
         with pytest.raises(RuntimeError if ok else ValueError, match="CUDA" if ok else "pool"):
             R.ragged_append(rows, rows, kp, vp, slots)
+
+
+def test_meta_shapes_of_the_torch_ops():
+    i = lambda *shape: torch.empty(*shape, dtype=torch.int64, device="meta")  # noqa: E731
+    got = torch.ops.razorkv.ragged_page_tables(i(3), i(3), i(3, 7), i(20), i(3), 16, 40)
+    assert [tuple(t.shape) for t in got] == [(3,), (40,), (40,), (4,), (3,)]
+    assert all(t.dtype == torch.int64 and t.device.type == "meta" for t in got)
+    x = lambda *shape: torch.empty(*shape, dtype=torch.bfloat16, device="meta")  # noqa: E731
+    assert torch.ops.razorkv.ragged_append(x(4, 2, 8), x(4, 2, 8), x(9, 2, 16, 8), x(9, 2, 16, 8), i(4)) is None
+    out, lse = torch.ops.razorkv.ragged_decode_attention(x(3, 4, 1, 8), x(9, 2, 16, 8), x(9, 2, 16, 8), i(3, 7), i(3))
+    assert out.shape == (3, 4, 1, 8) and out.dtype == torch.bfloat16
+    assert lse.shape == (3, 4) and lse.dtype == torch.float32
