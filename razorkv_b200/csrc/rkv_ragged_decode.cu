@@ -660,9 +660,9 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) issue(s);
 
-        // column x of head block n: the logit (unscaled, as they all are) that is the base, the one
-        // that renews it (-inf: none seen), and this lane's share of the sum
-        float o[DP / 16][NH][4], base[NH][2], limit[NH][2], l[NH][2];
+        // column x of head block n: the logit (unscaled, as they all are) that is the base, and this
+        // lane's share of the sum (zero: no logit seen)
+        float o[DP / 16][NH][4], base[NH][2], l[NH][2];
         auto reset = [&]() {
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
@@ -671,7 +671,7 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) o[d][n][x] = 0.f;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) { base[n][x] = 0.f; limit[n][x] = -INFINITY; l[n][x] = 0.f; }
+                for (int x = 0; x < 2; ++x) { base[n][x] = -FLT_MAX; l[n][x] = 0.f; }
             }
         };
         reset();
@@ -736,7 +736,7 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
                     float v = fmaxf(s[0][n][x], s[0][n][x + 2]);
                     if constexpr (TT == 32) v = fmaxf(v, fmaxf(s[1][n][x], s[1][n][x + 2]));
                     top[n][x] = v;
-                    over = over || v > limit[n][x];
+                    over = over || v > base[n][x] + slack;
                 }
             }
             if (__any_sync(0xffffffffu, over)) {
@@ -748,11 +748,10 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                        const bool renew = v > limit[n][x];
+                        const bool renew = v > base[n][x] + slack;
                         const float alpha =
-                            !renew ? 1.f : limit[n][x] == -INFINITY ? 0.f : sm100::ex2((base[n][x] - v) * scale2);
+                            !renew ? 1.f : sm100::ex2((base[n][x] - v) * scale2);
                         base[n][x] = renew ? v : base[n][x];
-                        limit[n][x] = renew ? v + slack : limit[n][x];
                         l[n][x] *= alpha;
 #pragma unroll
                         for (int d = 0; d < DP / 16; ++d) {
@@ -850,7 +849,7 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
                     for (int x = 0; x < 2; ++x) {
                         const float sum = l[n][x];
                         const int row = 8 * n + c2 + x;
-                        const float b = limit[n][x] == -INFINITY ? -INFINITY : base[n][x];
+                        const float b = l[n][x] == 0.f ? -INFINITY : base[n][x];
                         if (g == 0 && row < ng) {
                             if (!whole) { part.top(row) = b; part.sum(row) = sum; }
                             else if (p.lse) p.lse[(int64_t)get.b * p.Hq + h * G + g0 + row] = lse_of(p, b, sum);
