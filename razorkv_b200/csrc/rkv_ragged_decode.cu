@@ -67,24 +67,25 @@ __device__ __forceinline__ int64_t tiles_of(int64_t first, int64_t last) {
 
 // What a segment costs besides its tiles, in tiles: its queries, its outputs, the change of
 // pages.  Runs are of equal cost, so a segment of n tiles has n + over_of(TT) units, the first of
-// which hold no tile.  (64 requests of 1 to 4093 tokens: 38.7 us with 1, 38.2 with 2, 36.8 with 3
-// tiles of 16; 255 of up to 509: 26.3 us with 1, 28.4 with 2 tiles of 32.)
+// which hold no tile.  With 1, 2 and 3 of them, tiles of 16 (16 heads on each of 2 x 128): 64 requests
+// of up to 3000 tokens 22.4, 20.3 and 20.1 us, 8 of 18310 39.2, 37.7 and 38.6; tiles of 32: 64 of up to
+// 4093 (8 heads x 128) 34.5, 34.0 and 33.9, 255 of up to 509 (16 x 64) 24.2, 25.8 and 27.4.
 __host__ __device__ constexpr int over_of(int tile_tokens) { return tile_tokens <= 16 ? 2 : 1; }
 
 // Segments of so few tiles are not split between warps, or between CTAs: the boundary between two
 // runs moves to the nearer end of its segment.  Where no segment can have more tiles than are
 // split between CTAs, merge_kernel is not launched.
 // With at least half as many segments as warps, moving boundaries costs less balance than parts
-// cost joins: 64 requests of 250 tokens (8 kv heads x 128, 8 tiles) take 15.6 us whole and 22.8
-// split, 64 of 500 28.9 and 34.6; limits of 12 and 16 tiles for warps cost requests of mixed
-// lengths more than they gave (255 of 1 to 509 tokens, 16 heads x 64: 24.5 us, 27 and 27.6).
+// cost joins: 64 requests of 250 tokens (8 kv heads x 128, 8 tiles) take 15.7 us whole and 23.1
+// split, 64 of 500 28.8 and 34.8; limits of 12 and 16 tiles for warps cost requests of mixed
+// lengths more than they gave (255 of 0 to 509 tokens, 16 heads x 64: 24.2 us, 26.6 and 26.8).
 // With fewer, a segment has a CTA to itself if `most`, the tiles that the page table has room for,
-// are at most two per warp: 8 requests of 250 tokens (8 heads x 128) take 8.5 us, 10.1 with a limit
-// of four tiles for both, 1 of 77 6.3 and 6.9, 1 of 256 8.1 and 8.9.  Up to four tiles per warp, 1
-// of 500 takes 10.8 us instead of 9.1; split between warps from two tiles on, not three, 1 of 64
-// takes 6.6 us instead of 6.0.  Where other segments may be longer, this keeps a CTA at what all
+// are at most two per warp: 8 requests of 250 tokens (8 heads x 128) take 8.6 us, 10.3 with a limit
+// of four tiles for both, 1 of 77 6.6 and 7.2, 1 of 256 8.3 and 9.6.  Up to four tiles per warp, 1
+// of 500 takes 10.9 us instead of 9.3; split between warps from two tiles on, not three, 1 of 64
+// takes 6.8 us instead of 6.1.  Where other segments may be longer, this keeps a CTA at what all
 // could share (5 requests of up to 9001 tokens in fp32, 4 heads x 64, windows of 1 to 5000: 11.9 us
-// instead of 10.6).
+// instead of 10.7).
 struct Whole {
     int warp, cta;
 };
@@ -455,18 +456,18 @@ struct Walk {
 // takes half the registers.  P^T gets from the accumulator's layout to the operand's by an 8x8
 // transpose in registers.
 // Rounding P to 16 bits alone would add an error as large as the output's own rounding, so P
-// goes in as hi + lo, both 16-bit (with 16 heads, where products cost most, 19.7 us instead of
-// 19.1 for 16 requests of up to 16384 tokens).  The base of the power is a maximum seen so far that is
-// only renewed when a logit exceeds it by more than kSlack (in exponents of two), which saves the
-// reduction over lanes on most tiles; weights are then at most 2^kSlack instead of 1.  In fp16 they
-// are scaled by 2^kBias besides, so that small ones stay in fp16's normal range; that scale is taken
-// out of the log-sum-exp and cancels in the output.
+// goes in as hi + lo, both 16-bit (with 16 heads, where products cost most, 19.6 us instead of
+// 19.4 for 16 requests of up to 16384 tokens, 37.7 and 37.2 for 8 of 18310).  The base of the power
+// is a maximum seen so far that is only renewed when a logit exceeds it by more than kSlack (in
+// exponents of two), which saves the reduction over lanes on most tiles; weights are then at most
+// 2^kSlack instead of 1.  In fp16 they are scaled by 2^kBias besides, so that small ones stay in
+// fp16's normal range; that scale is taken out of the log-sum-exp and cancels in the output.
 // Rows outside the request's range are filled with zeros without being read: what the pool
 // holds there (NaN included) never enters a product.
 // Bound by memory: 8 requests of 32768 tokens (8 x 128, bf16) take 181 us, 5.9 TB/s of K and V,
 // 1 of 131072 (4 x 128) 53 us, 5.1 TB/s; about 7 us of a call are not: its launches, the sums over
-// the requests, the first tile's way, the joins.  Tensor pipes stay below a tenth of their rate up
-// to 8 heads per kv head; 16 heads reach 4.8 TB/s.
+// the requests, the first tile's way, the joins.  Tensor pipes are active an eighth of the time with
+// 7 heads per kv head; 16 heads reach 4.0 TB/s (8 requests of 18310 tokens, 2 x 128).
 // ------------------------------------------------------------------------------------------
 // 16 bytes, or zeros without a read
 __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool on) {
@@ -507,9 +508,9 @@ constexpr float tc_bias(bool bf16) { return bf16 ? 0.f : 6.f; }
 // Sums of the infinite and NaN elements of V over the tokens [t0, t1) of a request, for dims
 // 8 i + lane / 4 (zero where a column has none): what such a column of the output is, whatever the
 // (positive) weights are.  The products give NaN for it, since the low half of a weight may be zero
-// or negative.  Read again from the pool, by calls of such values only (the check costs 0.1 us of one
-// short request's 6.5, 0.4 us of 16 requests of up to 16384 tokens, 16 heads on each of 2 x 128).  The
-// four lanes of a dim share the tokens.
+// or negative.  Read again from the pool, by calls of such values only (the check costs 0.1 to 0.4 us
+// of a call: one short request 6.4 and 6.6, 64 of 500 tokens, 16 heads on each of 2 x 128, 20.9 and
+// 21.3).  The four lanes of a dim share the tokens.
 template <bool kBf16, int DP>
 __device__ __noinline__ void odd_columns(float (&sum)[DP / 8], const void* v, const int64_t* table, int64_t num_slots,
                                          int64_t P, int64_t stride_p, int64_t stride_t, int t0, int t1, int D) {
@@ -534,8 +535,8 @@ __device__ __noinline__ void odd_columns(float (&sum)[DP / 8], const void* v, co
     }
 }
 
-// kWhole: pages hold a multiple of 16 tokens, so 16 rows have one page (8 requests of 18310 tokens,
-// 96 dims and 16 heads on each of 4: 67 us, 71 with a page per row).
+// kWhole: pages hold a multiple of 16 tokens, so 16 rows have one page (16 requests of up to 16384
+// tokens, 16 heads on each of 2 x 128: 19.6 us, 20.1 with a page per row; long ones alike).
 template <bool kBf16, int DP, int NH, int TT, int NW, int STAGES, bool kWhole>
 __global__ void __launch_bounds__(NW * 32, 1)
 decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
@@ -911,15 +912,16 @@ decode_tc_kernel(DecodeParams p, int groups, Whole upto) {
 // fewer bits).  For the logits, LPT lanes share a token and read its row a quarter (half) each,
 // the queries come as broadcasts; for the output, a lane has DP / 32 dims of every head.  Both
 // halves are fused multiply-adds on pairs.  Up to 4 heads per kv head memory is the bound (8
-// requests of 9155 tokens, 4 kv heads x 128: 54 us, 5.5 TB/s), with 8 the instructions are (67 us).
+// requests of 9155 tokens, 4 kv heads x 128: 54 us, 5.6 TB/s), with 8 the instructions are (72 us).
 // ------------------------------------------------------------------------------------------
 template <int DP, int HG, int TT, int NW, int STAGES>
 struct F32Shape {
     static constexpr int kLpt = 32 / TT;                // lanes per token
     static constexpr int kPitch = DP * 4 + 16 * kLpt;   // 8 lanes at a time read 128 different bytes
     static constexpr int kPlane = TT * kPitch;
-    // Queries come with the first tile of their segment; with 8 heads they would take the room of
-    // two warps, and are read when the segment begins (8 requests of 9155 tokens, 4 kv heads x 128: 88 and 77 us).
+    // Queries come with the first tile of their segment; with 8 heads of 256 dims there is no room for
+    // them, and 8 heads read them when the segment begins (8 requests of 9155 tokens, 4 kv heads x 128:
+    // 72.2 us, where they would fit, and take 69.3, with the tile).
     static constexpr bool kQInRing = HG <= 4;
     static constexpr int kStage = 2 * kPlane + (kQInRing ? HG * kPitch : 0);
     static constexpr int kSmem = NW * (STAGES * kStage + HG * kPitch);
@@ -1466,10 +1468,11 @@ cudaError_t launch_pair(int threads, int smem, const DecodeParams& p, int HG, in
 template <bool kBf16, int DP, int NH, bool kWhole>
 cudaError_t launch_tc(const DecodeParams& p, cudaStream_t st) {
     // Tiles of 16 KB of K and V a warp and two of them in its ring: 128 KB on their way per SM, where
-    // 64 KB do not fill the memory (8 requests of 32768 tokens, 8 x 128: 207 us, 181 with 128 KB, 187
-    // with 256).  Four warps leave fewer parts to join than eight (1 request of 131072 tokens, 4 x 128:
-    // 53 and 57 us; 64 of 250, 8 x 128: 15.6 and 22.1), but 16 heads at a time are more work per tile
-    // than one warp per scheduler does in time (64 requests of 500 tokens, 2 x 128: 23.1 and 21.4).
+    // 64 KB do not fill the memory (8 requests of 32768 tokens, 8 x 128: 181 us, and 208 with tiles of 16
+    // tokens).  Four warps leave fewer parts to join than eight with tiles of 16 (1 request of 131072
+    // tokens, 4 x 128: 53 and 56 us; 64 of 250, 8 x 128: 15.7 and 19.1), but 16 heads at a time are more
+    // work per tile than one warp per scheduler does in time (64 requests of 500 tokens, 2 x 128: 23.9
+    // and 21.2).
     constexpr bool kWide = DP == 128 && NH == 2;
     constexpr int TT = DP <= 128 && !kWide ? 32 : 16, NW = DP <= 64 || kWide ? 8 : 4, STAGES = 2;
     using Shape = TcShape<DP, NH, TT, NW, STAGES>;
@@ -1502,7 +1505,7 @@ bool f32_ok(const DecodeParams& p) {
 
 template <int DP, int HG>
 cudaError_t launch_f32(const DecodeParams& p, cudaStream_t st) {
-    // (8 heads x 128: 67 us with four warps and tiles of 16 tokens, 77 with eight and 8)
+    // (8 heads x 128: 72 us with four warps and tiles of 16 tokens, 76 with eight and 8)
     constexpr bool kWide = DP == 128 && HG == 8;
     constexpr int TT = DP <= 64 || kWide ? 16 : 8, NW = DP <= 128 && !kWide ? 8 : 4, STAGES = 2;
     using Shape = F32Shape<DP, HG, TT, NW, STAGES>;

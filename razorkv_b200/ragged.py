@@ -119,8 +119,8 @@ def ragged_decode_attention(
     lengths [B] int64: request b attends its tokens ``starts[b] <= t < lengths[b]`` (from the
     first where ``starts`` is None; a sliding window or left padding otherwise), token t in
     row ``t % P`` of page ``page_table[b, t // P]``.  Returns [B, H, 1, D] in the query's dtype
-    (in ``out`` where given, which must not overlap what is read), and with ``return_lse`` also log sum exp(scale * q . k) as fp32
-    [B, H].  A request without such a token (a padded batch) gives zeros and -inf, and what the
+    (in ``out`` where given, which must not overlap what is read), and with ``return_lse`` also
+    log sum exp(scale * q . k) as fp32 [B, H].  A request without such a token (a padded batch) gives zeros and -inf, and what the
     pool holds elsewhere has no effect; infinities and NaN in attended rows take the formula's
     way into the output (an infinite element of V makes its column infinite, or NaN where both
     signs meet).  ``scale`` defaults to 1 / sqrt(D).
